@@ -328,6 +328,51 @@ int nvfp4_comfy_finish_scale(const float* amax, float* scale, nvfp4_stream_t str
 int nvfp4_comfy_rope(const void* x, const void* rotation, void* out, int64_t rows, int heads, int dim, int pairs, int backward,
                      nvfp4_stream_t stream);
 
+/*
+ * ---- the block of an image / video transformer ------------------------------------------------------------------------
+ * Layer norm with the residual sum in front of it and rotary positions over several axes; the reference leaves both to PyTorch
+ * (src/nvfp4_training/_workloads/lm.py).  `amax` arguments as above.
+ *
+ * nvfp4_layer_norm: total = x + delta (rounded to x's type; delta nullable, total is then x itself and sum_out unused),
+ *   h = (total - mean) * rstd * weight + bias with mean and rstd = 1 / sqrt(var + eps) over the cols elements of a row, all in
+ *   FP32.  x, total: FP32, BF16 or FP16; delta: x's type, or BF16 beside FP32; h: x's type, or BF16 beside FP32; weight, bias
+ *   (each nullable) of one type of the three.  Row pitches in elements; total and h are written contiguously.  mean_out,
+ *   rstd_out: FP32 [rows], nullable together (kept for the backward pass).
+ * nvfp4_layer_norm_bwd: with z = (total - mean) * rstd and u = dh * weight,
+ *   dx = rstd * (u - mean(u) - z * mean(u z)) (+ dsum, the gradient that arrives at total itself; nullable), written in
+ *   total's type and, where ddelta is given, in BF16 as well; dweight = sum over rows of dh * z, dbias = sum of dh (each
+ *   nullable), added in a fixed order through `partial`, FP32 scratch of nvfp4_layer_norm_bwd_partials(...) x 2 * cols.
+ */
+int nvfp4_layer_norm(const void* x, int x_dtype, int64_t x_pitch, const void* delta, int delta_dtype, int64_t delta_pitch,
+                     const void* weight, const void* bias, int weight_dtype, float eps, int64_t rows, int64_t cols, void* sum_out,
+                     void* h_out, int h_dtype, float* mean_out, float* rstd_out, float* amax, nvfp4_stream_t stream);
+int64_t nvfp4_layer_norm_bwd_partials(int64_t rows, int64_t cols);
+int nvfp4_layer_norm_bwd(const void* dh, int h_dtype, int64_t dh_pitch, const void* total, int x_dtype, int64_t total_pitch,
+                         const float* mean, const float* rstd, const void* weight, int weight_dtype, const void* dsum,
+                         int64_t dsum_pitch, int64_t rows, int64_t cols, void* dx, void* ddelta, float* partial, void* dweight,
+                         void* dbias, float* amax, nvfp4_stream_t stream);
+
+/*
+ * nvfp4_rotary_axes: up to three tensors [batch][seq][heads][dim] (strides of batch, seq and head in elements, features
+ *   contiguous) in one launch.  Pair j < pairs of a head turns by position[token][axis[j]] * turns[j] full turns, formed and
+ *   reduced in FP64; features from 2 * pairs on, and tensors with turn == 0, are copied.  interleaved: pair j is (2j, 2j + 1),
+ *   else (j, j + pairs).  inverse turns the other way (the backward pass).  positions: int64 (position_kind 0), int32 (1),
+ *   FP32 (2) or FP64 (3) with strides of batch, seq and axis in elements.  turns (FP64, frequency / 2 pi) and axis (uint8):
+ *   host arrays of `pairs` entries, at most NVFP4_ROTARY_MAX_PAIRS.
+ */
+enum { NVFP4_ROTARY_MAX_PAIRS = 256 };
+typedef struct {
+    const void* x;
+    void* out;
+    int64_t x_stride[3];   /* batch, seq, head */
+    int64_t out_stride[3];
+    int32_t heads;
+    int32_t turn;
+} nvfp4_rotary_tensor;
+int nvfp4_rotary_axes(const nvfp4_rotary_tensor* tensors, int count, int dtype, int64_t batch, int64_t seq, int dim,
+                      const void* positions, int position_kind, const int64_t* position_stride, int axes, const double* turns,
+                      const uint8_t* axis, int pairs, int interleaved, int inverse, float* amax, nvfp4_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

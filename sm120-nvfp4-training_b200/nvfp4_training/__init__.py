@@ -9,9 +9,10 @@ from ._runtime import load_runtime
 __all__ = ["list_profiles", "prepare_training", "enable_nvfp4", "train_step", "capture_step", "save_checkpoint", "load_checkpoint",
            "check_finite", "enable_lora", "prepare_lora", "lora_parameters", "save_lora", "load_lora", "merge_lora",
            "capture_lora_step", "PackedNVFP4Linear", "pack_frozen_layers", "save_frozen_cache", "load_frozen_cache", "capture_frozen",
-           "enable_data_parallel"]
+           "enable_data_parallel", "layer_norm", "add_layer_norm", "LayerNorm", "rotary_axes", "rotary_axes_qkv"]
 
 _LORA = {"enable_lora", "prepare_lora", "lora_parameters", "save_lora", "load_lora", "merge_lora", "PackedNVFP4Linear", "capture_lora_step"}
+_OPERATORS = {"layer_norm", "add_layer_norm", "LayerNorm", "rotary_axes", "rotary_axes_qkv"}
 
 
 def __getattr__(name):
@@ -19,6 +20,10 @@ def __getattr__(name):
     if name in _LORA:
         from . import lora
         return getattr(lora, name)
+    if name in _OPERATORS:
+        from . import operators
+        globals()[name] = getattr(operators, name)
+        return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 

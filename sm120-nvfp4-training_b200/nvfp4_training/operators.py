@@ -1,0 +1,335 @@
+"""Operators of an image / video transformer block: layer norm with the residual sum in front of it, and rotary positions over
+several axes.  The kernels are nvfp4_layer_norm / nvfp4_layer_norm_bwd and nvfp4_rotary_axes of the C-ABI library; everything
+here is differentiable once and may be captured into a CUDA graph.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from functools import lru_cache
+
+import torch
+from torch import nn
+
+from . import _native as nat
+from ._backend.quant import attach_amax
+
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _check_tensor(name, t, dtypes=_FLOATS):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if t.dtype not in dtypes:
+        raise TypeError(f"Unsupported dtype {t.dtype} of {name}")
+
+
+def _check_device(t):
+    """Last of an operator's checks: the arguments fit together, now they also have to be on a GPU."""
+    if not t.is_cuda:
+        raise ValueError("This operator needs CUDA tensors")
+
+
+def _zeroed_slot(device):
+    """float32[4] in the layout of nat.amax for one result; its own zero fill, so that a graph which records it replays it."""
+    return torch.zeros(4, dtype=torch.float32, device=device)
+
+
+# ---- layer norm -------------------------------------------------------------------------------------------------------
+def _rows(t, cols):
+    """[rows, cols] view with contiguous rows (any row pitch); a copy only where the layout has no such view."""
+    flat = t.reshape(-1, cols)
+    if (cols > 1 and flat.stride(1) != 1) or (flat.shape[0] > 1 and flat.stride(0) < cols):
+        flat = flat.contiguous()
+    return flat
+
+
+def _pitch(flat):
+    return max(flat.stride(0), flat.shape[1])
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, delta, weight, bias, eps, out_dtype, want_amax):
+        shape, cols, dev = x.shape, x.shape[-1], x.device
+        x2 = _rows(x, cols)
+        d2 = None if delta is None else _rows(delta, cols)
+        rows = x2.shape[0]
+        total = x2 if d2 is None else torch.empty((rows, cols), dtype=x.dtype, device=dev)
+        h = torch.empty((rows, cols), dtype=out_dtype, device=dev)
+        stats = torch.empty((2, rows), dtype=torch.float32, device=dev)
+        amax = _zeroed_slot(dev) if want_amax else None
+        affine = weight if weight is not None else bias
+        wcode = 0 if affine is None else nat.dtype_code(affine)
+        if rows:
+            with torch.cuda.device(dev):
+                nat.check(nat.lib().nvfp4_layer_norm(
+                    x2.data_ptr(), nat.dtype_code(x2), _pitch(x2), nat.ptr(d2), 0 if d2 is None else nat.dtype_code(d2),
+                    0 if d2 is None else _pitch(d2), nat.ptr(weight), nat.ptr(bias), wcode, eps, rows, cols,
+                    None if d2 is None else total.data_ptr(), h.data_ptr(), nat.dtype_code(h), stats[0].data_ptr(), stats[1].data_ptr(),
+                    nat.ptr(amax), nat.stream_of(x)))
+        ctx.save_for_backward(total, stats, weight)
+        ctx.delta_dtype, ctx.shape, ctx.want_amax = None if delta is None else delta.dtype, shape, want_amax
+        ctx.affine = (weight is not None and ctx.needs_input_grad[2], bias is not None and ctx.needs_input_grad[3],
+                      None if affine is None else affine.dtype)
+        ctx.set_materialize_grads(False)
+        if amax is not None:
+            ctx.mark_non_differentiable(amax)
+        return (None if d2 is None else total.view(shape)), h.view(shape), amax
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dsum, dh, _):
+        total, stats, weight = ctx.saved_tensors
+        rows, cols = total.shape
+        dev = total.device
+        need_w, need_b, wdtype = ctx.affine
+        if dh is None:       # only the residual path carries a gradient
+            dd = None if (dsum is None or ctx.delta_dtype is None) else dsum.to(ctx.delta_dtype)
+            zero = torch.zeros(cols, dtype=wdtype, device=dev) if (need_w or need_b) else None
+            return dsum, dd, (zero if need_w else None), (zero if need_b else None), None, None, None
+        g = _rows(dh, cols)
+        res = None if dsum is None else _rows(dsum, cols)
+        dx = torch.empty((rows, cols), dtype=total.dtype, device=dev)
+        narrow = ctx.delta_dtype is not None and ctx.delta_dtype != total.dtype
+        dd = torch.empty((rows, cols), dtype=ctx.delta_dtype, device=dev) if narrow else None
+        dw = torch.empty(cols, dtype=wdtype, device=dev) if need_w else None
+        db = torch.empty(cols, dtype=wdtype, device=dev) if need_b else None
+        amax = _zeroed_slot(dev) if ctx.want_amax and (narrow or total.dtype == torch.bfloat16) else None
+        if rows:
+            partial = None
+            if need_w or need_b:
+                parts = int(nat.lib().nvfp4_layer_norm_bwd_partials(rows, cols))
+                partial = torch.empty((parts, 2, cols), dtype=torch.float32, device=dev)
+            with torch.cuda.device(dev):
+                nat.check(nat.lib().nvfp4_layer_norm_bwd(
+                    g.data_ptr(), nat.dtype_code(g), _pitch(g), total.data_ptr(), nat.dtype_code(total), _pitch(total), stats[0].data_ptr(),
+                    stats[1].data_ptr(), nat.ptr(weight), 0 if wdtype is None else nat._CODES[wdtype], nat.ptr(res), 0 if res is None else _pitch(res),
+                    rows, cols, dx.data_ptr(), nat.ptr(dd), nat.ptr(partial), nat.ptr(dw), nat.ptr(db), nat.ptr(amax), nat.stream_of(total)))
+        else:
+            for t in (dw, db):
+                if t is not None:
+                    t.zero_()
+        dx = dx.view(ctx.shape)
+        dd = dd.view(ctx.shape) if narrow else (dx if ctx.delta_dtype is not None else None)
+        if amax is not None:
+            attach_amax(dd if narrow else dx, amax)
+        return dx, dd, dw, db, None, None, None
+
+
+def _layer_norm(x, delta, weight, bias, eps, out_dtype, want_amax=False):
+    _check_tensor("x", x)
+    if x.ndim == 0 or x.shape[-1] == 0:
+        raise ValueError("layer norm needs a last dimension of at least one feature")
+    cols = x.shape[-1]
+    eps = float(eps)
+    if not (math.isfinite(eps) and eps >= 0):
+        raise ValueError("eps must be finite and not negative")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype != x.dtype and not (x.dtype == torch.float32 and out_dtype == torch.bfloat16):
+        raise TypeError("the result has the input's dtype, or BF16 beside an FP32 input")
+    if delta is not None:
+        _check_tensor("delta", delta)
+        if delta.dtype != x.dtype and not (x.dtype == torch.float32 and delta.dtype == torch.bfloat16):
+            raise TypeError("delta has the input's dtype, or BF16 beside an FP32 input")
+        if delta.shape != x.shape or delta.device != x.device:
+            raise ValueError("x and delta must have one shape and device")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None:
+            _check_tensor(name, p)
+            if p.shape != (cols,) or p.device != x.device or not p.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous vector of the last dimension's {cols} features on the input's device")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError("weight and bias must have one dtype")
+    _check_device(x)
+    return _LayerNorm.apply(x, delta, weight, bias, eps, out_dtype, want_amax and out_dtype == torch.bfloat16)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, *, out_dtype=None):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension.  x: FP32, BF16 or FP16 with any strides; weight
+    and bias (each optional) of one floating dtype.  out_dtype: x's, or torch.bfloat16 beside an FP32 x, which is what an
+    NVFP4 or 8-bit layer reads.  Statistics are FP32."""
+    return _layer_norm(x, None, weight, bias, eps, out_dtype)[1]
+
+
+def add_layer_norm(x, delta, weight=None, bias=None, eps=1e-5, *, out_dtype=None):
+    """(total, layer_norm(total)) with total = x + delta rounded to x's dtype: the residual sum of a transformer block and
+    the norm behind it in one pass.  delta has x's dtype, or BF16 beside an FP32 x (a layer's output under autocast)."""
+    if delta is None:
+        raise TypeError("delta must be a tensor; use layer_norm without one")
+    return _layer_norm(x, delta, weight, bias, eps, out_dtype)[:2]
+
+
+class LayerNorm(nn.LayerNorm):
+    """nn.LayerNorm over the last dimension on this library's kernels (same parameters and state dict).  Under CUDA BF16
+    autocast an FP32 input gives a BF16 result, which is what the next converted layer reads; BF16 results carry their amax."""
+
+    def forward(self, x):
+        out = torch.bfloat16 if (x.dtype == torch.float32 and torch.is_autocast_enabled("cuda")
+                                 and torch.get_autocast_dtype("cuda") == torch.bfloat16) else x.dtype
+        _, h, amax = _layer_norm(x, None, self.weight, self.bias, self.eps, out, want_amax=True)
+        return h if amax is None else attach_amax(h, amax)
+
+
+# ---- rotary positions over several axes -----------------------------------------------------------------------------------
+_POSITION_KINDS = {torch.int64: 0, torch.int32: 1, torch.float32: 2, torch.float64: 3}
+MAX_PAIRS = 256
+
+
+class _Tensor(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("x_stride", C.c_int64 * 3), ("out_stride", C.c_int64 * 3), ("heads", C.c_int32),
+                ("turn", C.c_int32)]
+
+
+@lru_cache(maxsize=256)
+def _plan(sections, theta, frequencies):
+    """Host arrays for the kernel: frequency / (2 pi) and axis of every pair."""
+    pairs = sum(sections)
+    turns, axis = (C.c_double * pairs)(), (C.c_uint8 * pairs)()
+    j = 0
+    for a, n in enumerate(sections):
+        for i in range(n):
+            exponent = i / n if frequencies == "axis" else j / pairs
+            turns[j] = theta ** -exponent / (2 * math.pi)
+            axis[j] = a
+            j += 1
+    return turns, axis, pairs
+
+
+def _launch_rotary(jobs, positions, plan, axes, dim, interleaved, inverse, amax):
+    """jobs: (x, out, turn), each [batch, seq, heads, dim] with contiguous features."""
+    x0 = jobs[0][0]
+    turns, axis, pairs = plan
+    tensors = (_Tensor * len(jobs))()
+    for t, (x, out, turn) in zip(tensors, jobs):
+        t.x, t.out, t.heads, t.turn = x.data_ptr(), out.data_ptr(), x.shape[2], int(turn)
+        t.x_stride[:], t.out_stride[:] = x.stride()[:3], out.stride()[:3]
+    ps = (0,) * (3 - positions.ndim) + positions.stride()
+    with torch.cuda.device(x0.device):
+        nat.check(nat.lib().nvfp4_rotary_axes(tensors, len(jobs), nat.dtype_code(x0), x0.shape[0], x0.shape[1], dim, positions.data_ptr(),
+                                              _POSITION_KINDS[positions.dtype], (C.c_int64 * 3)(*ps), axes, turns, axis, pairs,
+                                              int(interleaved), int(inverse), nat.ptr(amax), nat.stream_of(x0)))
+
+
+def _features_contiguous(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+class _RotaryAxes(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, plan, axes, interleaved):
+        ctx.save_for_backward(positions)
+        ctx.how = (plan, axes, interleaved)
+        ctx.set_materialize_grads(False)
+        sources = [t for t in (q, k) if t is not None]
+        outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in sources]
+        if sources[0].numel():
+            _launch_rotary([(_features_contiguous(t), o, True) for t, o in zip(sources, outs)], positions, plan, axes, q.shape[3], interleaved, False, None)
+        return outs[0], (outs[1] if k is not None else None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        positions, = ctx.saved_tensors
+        plan, axes, interleaved = ctx.how
+        grads = [None if g is None else torch.empty(g.shape, dtype=g.dtype, device=g.device) for g in (dq, dk)]
+        jobs = [(_features_contiguous(g), o, True) for g, o in zip((dq, dk), grads) if g is not None and g.numel()]
+        if jobs:
+            _launch_rotary(jobs, positions, plan, axes, jobs[0][0].shape[3], interleaved, True, None)
+        return grads[0], grads[1], None, None, None, None
+
+
+class _RotaryFused(torch.autograd.Function):
+    """q and k of a fused projection rotated into tensors of their own, v a view of the projection; backward puts the three
+    gradients together in one launch."""
+
+    @staticmethod
+    def forward(ctx, qkv, positions, plan, axes, interleaved, heads, kv_heads):
+        b, s, width = qkv.shape
+        d = width // (heads + 2 * kv_heads)
+        ctx.save_for_backward(positions)
+        ctx.how, ctx.dims = (plan, axes, interleaved), (b, s, heads, kv_heads, d)
+        ctx.set_materialize_grads(False)
+        parts = qkv.detach().view(b, s, heads + 2 * kv_heads, d).split((heads, kv_heads, kv_heads), dim=2)
+        q = torch.empty((b, s, heads, d), dtype=qkv.dtype, device=qkv.device)
+        k = torch.empty((b, s, kv_heads, d), dtype=qkv.dtype, device=qkv.device)
+        if qkv.numel():
+            _launch_rotary([(parts[0], q, True), (parts[1], k, True)], positions, plan, axes, d, interleaved, False, None)
+        return q, k, parts[2]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk, dv):
+        positions, = ctx.saved_tensors
+        plan, axes, interleaved = ctx.how
+        b, s, heads, kv_heads, d = ctx.dims
+        some = next(g for g in (dq, dk, dv) if g is not None)
+        dqkv = torch.empty((b, s, (heads + 2 * kv_heads) * d), dtype=some.dtype, device=some.device)
+        amax = _zeroed_slot(some.device) if some.dtype == torch.bfloat16 else None
+        jobs = []
+        for g, o, turn in zip((dq, dk, dv), dqkv.view(b, s, -1, d).split((heads, kv_heads, kv_heads), dim=2), (True, True, False)):
+            if g is None:
+                o.zero_()
+            else:
+                jobs.append((_features_contiguous(g), o, turn))
+        if dqkv.numel():
+            _launch_rotary(jobs, positions, plan, axes, d, interleaved, True, amax)
+        return (dqkv if amax is None else attach_amax(dqkv, amax)), None, None, None, None, None, None
+
+
+def _check_rotary(x, batch, seq, dim, positions, sections, theta, layout, frequencies):
+    sections = tuple(sections)
+    if not sections or any(type(n) is not int or n < 1 for n in sections):
+        raise ValueError("sections must be positive integers: the pairs of a head that each position axis turns")
+    if 2 * sum(sections) > dim or sum(sections) > MAX_PAIRS:
+        raise ValueError(f"sections hold {sum(sections)} pairs; a head of {dim} features has room for {min(dim // 2, MAX_PAIRS)}")
+    if layout not in ("half", "interleaved"):
+        raise ValueError("layout must be 'half' or 'interleaved'")
+    if frequencies not in ("shared", "axis"):
+        raise ValueError("frequencies must be 'shared' or 'axis'")
+    theta = float(theta)
+    if not (math.isfinite(theta) and theta > 0):
+        raise ValueError("theta must be positive and finite")
+    _check_tensor("positions", positions, tuple(_POSITION_KINDS))
+    if positions.device != x.device or positions.shape not in ((seq, len(sections)), (batch, seq, len(sections))):
+        raise ValueError(f"positions must be [{seq}, {len(sections)}] or [{batch}, {seq}, {len(sections)}] on the input's device")
+    _check_device(x)
+    return _plan(sections, theta, frequencies), len(sections), layout == "interleaved"
+
+
+def rotary_axes(q, k, positions, sections, *, theta=10000.0, layout="half", frequencies="shared"):
+    """(q, k) turned by rotary positions over several axes; k may be None.  q [batch, seq, heads, dim], k [batch, seq,
+    kv_heads, dim] of one dtype (FP32, BF16, FP16) with any strides; positions [seq, axes] or [batch, seq, axes], int32,
+    int64, FP32 or FP64; sections: pairs turned by each axis, in order, at most dim / 2 in all (features behind the turned
+    ones pass unchanged).  frequencies 'shared': pair j of all P turns by theta^(-j / P), whatever its axis; 'axis': pair i
+    of an axis of n pairs by theta^(-i / n).  layout 'half': pair j is features (j, j + P); 'interleaved': (2j, 2j + 1).
+    Angles are FP64."""
+    _check_tensor("q", q)
+    if q.ndim != 4:
+        raise ValueError("q must be [batch, seq, heads, dim]")
+    if k is not None:
+        _check_tensor("k", k)
+        if k.dtype != q.dtype:
+            raise TypeError("q and k must have one dtype")
+        if k.ndim != 4 or k.device != q.device or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]:
+            raise ValueError("k must be [batch, seq, kv_heads, dim] beside q")
+        if k.shape[2] == 0:
+            raise ValueError("k needs at least one head")
+    if q.shape[2] == 0:
+        raise ValueError("q needs at least one head")
+    how = _check_rotary(q, q.shape[0], q.shape[1], q.shape[3], positions, sections, theta, layout, frequencies)
+    return _RotaryAxes.apply(q, k, positions, *how)
+
+
+def rotary_axes_qkv(qkv, positions, sections, heads, kv_heads=None, *, theta=10000.0, layout="half", frequencies="shared"):
+    """(q, k, v) of a fused projection qkv [batch, seq, (heads + 2 * kv_heads) * dim], q and k turned as by rotary_axes, v a
+    view of qkv.  The gradient of qkv is written in one pass over those of q, k and v."""
+    _check_tensor("qkv", qkv)
+    kv_heads = heads if kv_heads is None else kv_heads
+    if type(heads) is not int or type(kv_heads) is not int or heads < 1 or kv_heads < 1:
+        raise ValueError("heads and kv_heads must be positive integers")
+    if qkv.ndim != 3 or qkv.shape[2] == 0 or qkv.shape[2] % (heads + 2 * kv_heads):
+        raise ValueError("qkv must be [batch, seq, (heads + 2 * kv_heads) * dim]")
+    dim = qkv.shape[2] // (heads + 2 * kv_heads)
+    how = _check_rotary(qkv, qkv.shape[0], qkv.shape[1], dim, positions, sections, theta, layout, frequencies)
+    return _RotaryFused.apply(_features_contiguous(qkv), positions, *how, heads, kv_heads)
