@@ -373,6 +373,30 @@ int nvfp4_rotary_axes(const nvfp4_rotary_tensor* tensors, int count, int dtype, 
                       const void* positions, int position_kind, const int64_t* position_stride, int axes, const double* turns,
                       const uint8_t* axis, int pairs, int interleaved, int inverse, float* amax, nvfp4_stream_t stream);
 
+/*
+ * ---- 8-bit floating point ------------------------------------------------------------------------------------------------
+ * A linear layer's products with e4m3 operands and a power-of-two scale for each block of 128; no counterpart in the reference.
+ *
+ * nvfp4_fp8_quantize: e4m3 codes of x [rows][cols] (FP32, BF16 or FP16, row pitch in elements) with one power-of-two scale
+ *   2^e per block, e the smallest exponent with amax / 2^e <= 448, at least -127, and 0 for a block of zeros.  A block that
+ *   holds a value that is not finite has NaN for all of its codes.
+ *   codes [rows][cols_p], scales: blocks of 1 x 128 along the columns; codes_t [cols][rows_p], scales_t: the transposed
+ *   packing with blocks of 128 along the rows; either may be null.  square: blocks of 128 x 128, one scale for both packings.
+ *   rows_p, cols_p: rounded up to 128, the padding is written as zeros.  Scales are UE8M0 bytes, written four times each so
+ *   that every 32 elements of the contraction have one, in the 512-byte blocks of 128 rows x 4 of the NVFP4 packings:
+ *   [rows_p / 128][cols_p / 128][512] bytes (transposed: [cols_p / 128][rows_p / 128][512]).
+ *   column_sums (nullable): FP32 [rows_p / 128][cols], the sums of x over each 128 rows.
+ * nvfp4_fp8_gemm: out[M][N] = A B^T (+ bias[N]) on such packings, a [M][K], b [N][K], K a multiple of 128; FP32 accumulation,
+ *   one rounding to out's type (FP32, BF16 or FP16; bias of one of these types).  Row pitch ldo in elements.
+ * nvfp4_column_sums: out[cols] = sum over `parts` FP32 rows, added in a fixed order, in any of the three types.
+ */
+int nvfp4_fp8_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t pitch, int square, uint8_t* codes,
+                       uint8_t* scales, uint8_t* codes_t, uint8_t* scales_t, float* column_sums, nvfp4_stream_t stream);
+int nvfp4_fp8_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* b, const uint8_t* b_scales, int64_t M, int64_t N,
+                   int64_t K, const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo, int* status,
+                   nvfp4_stream_t stream);
+int nvfp4_column_sums(const float* partial, int64_t parts, int64_t cols, void* out, int out_dtype, nvfp4_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,563 @@
+// Products of e4m3 operands with a power-of-two scale per block of 128:  out[M][N] = (A o SA) (B o SB)^T (+ bias).
+//
+// tcgen05.mma.kind::mxf8f6f4 multiplies a UE8M0 scale into every 32 elements of the contraction; the packings give the four
+// 32-blocks of a 128-block the same byte, so the tensor cores apply the block scale themselves and accumulate over the whole
+// contraction in FP32 tensor memory, without a pass of multiply-adds per block on the CUDA cores.
+//
+// Two kernels.
+//   fp8_gemm_kernel        persistent clusters of two CTAs on 256 x 256 tiles (cta_group::2, M256 x N256 x K32 instructions), for
+//                          problems that fill the GPU with such tiles.  Tensor issue and the shared-memory bandwidth under
+//                          it are the bound.
+//   fp8_gemm_split_kernel  one 128 x 128 tile per cluster of 1 to 8 CTAs, each with a share of the contraction; the FP32
+//                          partial tiles are added through distributed shared memory in rank order.  For few rows (the weight
+//                          is read once, HBM or latency is the bound) and for problems of few tiles.
+// The host picks by the estimated number of cycles of each (split_for below).
+// Operands are unpadded in M and N: tile loads beyond the tensor arrive as zeros, stores are cropped.
+// Every wait is bounded as in the NVFP4 GEMM: on expiry the status word is raised, all roles leave, and the kernel returns.
+#include "async.cuh"
+#include "tcgen05.cuh"
+#include "vec.cuh"
+
+#include <algorithm>
+
+namespace nvfp4 {
+
+constexpr int G8_BK = 128;                  // elements (and bytes) of the contraction per stage: one scale block
+constexpr int G8_SF = 512;                  // bytes of a scale block: 128 rows x 4
+constexpr int G8_OPERAND = 128 * 128;       // bytes of 128 rows of an operand per stage
+
+struct Gemm8Args {
+    const void* bias;
+    void* out;
+    int* status;
+    int64_t ldo;
+    int bias_dtype, M, N, k_tiles, tiles_m, tiles_n, tma_store;
+};
+
+__device__ __forceinline__ uint32_t instr_desc8(int n, int m) {    // e4m3 x e4m3, UE8M0 scales, K-major A and B
+    return (1u << 23) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+template <bool PAIR>
+__device__ __forceinline__ void mma8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate, uint32_t tmem_sfa,
+                                     uint32_t tmem_sfb) {
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+            ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(tmem_sfa), "r"(tmem_sfb) : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+            ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(tmem_sfa), "r"(tmem_sfb) : "memory");
+}
+__device__ __forceinline__ float bias_at(const Gemm8Args& g, int64_t col) {
+    float b[1];
+    load_param<1>(g.bias, g.bias_dtype, col, b);
+    return b[0];
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const T lo = from_float<T>(a), hi = from_float<T>(b);
+    return static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(&lo)) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(&hi)) << 16;
+}
+
+// ====================================================================================================================
+// clusters of two on 256 x 256 tiles
+// ====================================================================================================================
+namespace pair8 {
+constexpr int THREADS = 320, EPI_WARPS = 8, FIRST_EPI_WARP = 2;
+constexpr int STAGES = 6;
+constexpr int OPERANDS = 2 * G8_OPERAND;             // this CTA's 128 rows of A and its 128 of the tile's 256 rows of B
+constexpr int SCALES = 3 * G8_SF;                    // this CTA's rows of A; all 256 rows of B
+constexpr int STAGE_BYTES = OPERANDS + SCALES;
+// Tensor memory: two accumulators of 256 columns that share 32 ([0, 256) and [224, 480)), so that two scale buffers of
+// 4 + 8 columns fit behind them.  The epilogue reads the shared columns first, and only that read gates the next tile.
+constexpr int ACC_STRIDE = 224, SF_BASE = 480, SF_COLS = 12, TMEM_COLS = 512;
+constexpr int SLAB = 1024;                           // 32 rows x 32 bytes per epilogue warp
+constexpr int BARS = 2 * STAGES + 4;
+constexpr int SMEM = STAGES * STAGE_BYTES + EPI_WARPS * SLAB + 1024 + 256;
+static_assert(SF_BASE + 2 * SF_COLS <= TMEM_COLS && BARS * 8 + 16 <= 256 && SMEM <= 232448, "budgets");
+}  // namespace pair8
+
+template <typename TO>
+__global__ void __launch_bounds__(pair8::THREADS, 1)
+fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_sfa,
+                const __grid_constant__ CUtensorMap map_sfb, const __grid_constant__ CUtensorMap map_out, const Gemm8Args g) {
+    using namespace pair8;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* epi_smem = smem + STAGES * OPERANDS;
+    uint8_t* sf_smem = epi_smem + EPI_WARPS * SLAB;
+    uint64_t* full = reinterpret_cast<uint64_t*>(sf_smem + STAGES * SCALES);
+    uint64_t* empty = full + STAGES;
+    uint64_t* acc_full = empty + STAGES;
+    uint64_t* shared_drained = acc_full + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(shared_drained + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const int rank = static_cast<int>(cluster_rank());
+    const bool leader = rank == 0;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int a = 0; a < 2; ++a) mbar_init(&acc_full[a], 1);
+        mbar_init(shared_drained, EPI_WARPS * 2);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int total_tiles = g.tiles_m * g.tiles_n;
+    const int first_tile = static_cast<int>(blockIdx.x >> 1), tile_step = static_cast<int>(gridDim.x >> 1);
+
+    if (warp == 0) {
+        // ---- loads: the whole warp runs the loop, one elected lane issues; both CTAs' bytes count on the leader's barrier ----
+        int stage = 0, issued = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int t = first_tile; t < total_tiles && ok; t += tile_step) {
+            const int tm = (t % g.tiles_m) * 2 + rank, tn = t / g.tiles_m;
+            for (int kt = 0; kt < g.k_tiles; ++kt) {
+                if (!mbar_wait_warp(&empty[stage], phase ^ 1, abort_flag)) { ok = false; break; }
+                if (elect_one()) {
+                    uint8_t* st = smem + stage * OPERANDS;
+                    uint8_t* sf = sf_smem + stage * SCALES;
+                    if (leader) mbar_expect_tx(&full[stage], 2 * STAGE_BYTES);
+                    tma_load_2d_pair(st, &map_a, kt * G8_BK, tm * 128, &full[stage]);
+                    tma_load_2d_pair(st + G8_OPERAND, &map_b, kt * G8_BK, tn * 256 + rank * 128, &full[stage]);
+                    tma_load_2d_pair(sf, &map_sfa, 0, tm * g.k_tiles + kt, &full[stage]);
+                    tma_load_2d_pair(sf + G8_SF, &map_sfb, 0, tn * 2 * g.k_tiles + kt, &full[stage]);
+                    tma_load_2d_pair(sf + 2 * G8_SF, &map_sfb, 0, (tn * 2 + 1) * g.k_tiles + kt, &full[stage]);
+                }
+                __syncwarp();
+                ++issued;
+                if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            }
+        }
+        if (!ok && lane == 0) {
+            // loads in flight still write into this CTA's shared memory: a bounded chance to land
+            const int pending = min(issued, STAGES);
+            for (int i = 0; i < pending; ++i) {
+                if (--stage < 0) { stage = STAGES - 1; phase ^= 1; }
+                const long long t0 = clock64();
+                if (leader) while (!mbar_try(&full[stage], phase) && clock64() - t0 < WAIT_CYCLES / 8) {}
+            }
+            const long long t0 = clock64();
+            while (clock64() - t0 < 400000) {}
+        }
+    } else if (warp == 1) {
+        // ---- MMA issue, by the leader for both CTAs; scale copies and MMAs execute in issue order ----
+        if (leader) {
+            const uint32_t idesc = instr_desc8(256, 256);
+            int stage = 0, local = 0, sf_buf = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int t = first_tile; t < total_tiles && ok; t += tile_step, ++local) {
+                const int acc = local & 1;
+                const uint32_t tmem_acc = tmem_base + acc * ACC_STRIDE;
+                if (local > 0) {       // the previous tile's shared columns are read, and with them everything of the tile before
+                    if (!mbar_wait_warp(shared_drained, (local - 1) & 1, abort_flag)) { ok = false; break; }
+                    tc_fence_after();
+                }
+                for (int kt = 0; kt < g.k_tiles; ++kt) {
+                    if (!mbar_wait_warp(&full[stage], phase, abort_flag)) { ok = false; break; }
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t sa = smem_u32(smem + stage * OPERANDS), sb = sa + G8_OPERAND, sf = smem_u32(sf_smem + stage * SCALES);
+                        const uint32_t tsfa = tmem_base + SF_BASE + sf_buf * SF_COLS, tsfb = tsfa + 4;
+                        tc_cp_sf_pair(tsfa, scale_desc(sf));
+                        tc_cp_sf_pair(tsfb, scale_desc(sf + G8_SF));
+                        tc_cp_sf_pair(tsfb + 4, scale_desc(sf + 2 * G8_SF));
+#pragma unroll
+                        for (int kb = 0; kb < 4; ++kb)
+                            mma8<true>(tmem_acc, operand_desc(sa + kb * 32), operand_desc(sb + kb * 32), idesc, (kt | kb) ? 1u : 0u, tsfa, tsfb);
+                        tc_commit_pair(&empty[stage]);
+                    }
+                    __syncwarp();
+                    sf_buf ^= 1;
+                    if (++stage == STAGES) { stage = 0; phase ^= 1; }
+                }
+                if (ok && elect_one()) tc_commit_pair(&acc_full[acc]);
+                __syncwarp();
+            }
+        }
+    } else {
+        // ---- epilogue: two warps per TMEM sub-partition, eight 16-column units of the tile each ----
+        constexpr int ESZ = sizeof(TO);
+        const int sub = warp & 3, half = (warp - FIRST_EPI_WARP) >> 2;
+        uint8_t* slab = epi_smem + (warp - FIRST_EPI_WARP) * SLAB;
+        int local = 0;
+        // 32 rows x 32 bytes, two uint4 per lane: through the staging slab and a TMA store (which crops), or directly
+        auto emit = [&](const uint4& q0, const uint4& q1, int64_t row, int64_t col0, int tile_row0) {
+            if (g.tma_store) {
+                if (lane == 0) bulk_wait_read<0>();
+                __syncwarp();
+                const int sw = (lane >> 2) & 1;
+                *reinterpret_cast<uint4*>(slab + lane * 32 + (sw << 4)) = q0;
+                *reinterpret_cast<uint4*>(slab + lane * 32 + ((1 ^ sw) << 4)) = q1;
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) { tma_store_2d(&map_out, static_cast<int>(col0), tile_row0, slab); bulk_commit(); }
+            } else if (row < g.M) {
+                TO* dst = static_cast<TO*>(g.out) + row * g.ldo + col0;
+                const uint32_t w[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
+#pragma unroll
+                for (int j = 0; j < 32 / ESZ; ++j)
+                    if (col0 + j < g.N) {
+                        if constexpr (ESZ == 4) reinterpret_cast<uint32_t*>(dst)[j] = w[j & 7];
+                        else reinterpret_cast<uint16_t*>(dst)[j] = static_cast<uint16_t>(w[j >> 1] >> ((j & 1) * 16));
+                    }
+            }
+        };
+        for (int t = first_tile; t < total_tiles; t += tile_step, ++local) {
+            const int tm = (t % g.tiles_m) * 2 + rank, tn = t / g.tiles_m;
+            const int acc = local & 1;
+            if (!mbar_wait(&acc_full[acc], (local >> 1) & 1, abort_flag)) break;
+            tc_fence_after();
+            const int tile_row0 = tm * 128 + sub * 32;
+            const int64_t row = tile_row0 + lane, colbase = static_cast<int64_t>(tn) * 256;
+            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(sub * 32) << 16) + acc * ACC_STRIDE;
+            // unit i of this warp: the shared one first (the last two of stage 0, the first two of stage 1), then seven of its own
+            auto unit_of = [&](int i) { return i == 0 ? (acc == 0 ? 14 + half : half) : (acc == 0 ? 0 : 2) + half * 7 + (i - 1); };
+            auto read = [&](int i, uint32_t (&r)[16]) {
+                tc_ld16(taddr + unit_of(i) * 16, r);
+                tc_wait_ld();
+                if (i == 0) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) { if (leader) mbar_arrive(shared_drained); else mbar_arrive_leader(shared_drained); }
+                }
+                if (g.bias) {
+                    const int64_t c0 = colbase + unit_of(i) * 16;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (c0 + j < g.N) r[j] = __float_as_uint(__uint_as_float(r[j]) + bias_at(g, c0 + j));
+                }
+            };
+            if constexpr (ESZ == 2) {      // drain to packed registers, then store
+                uint32_t packed[64];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    uint32_t r[16];
+                    read(i, r);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) packed[i * 8 + j] = pack2<TO>(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+                }
+                if (tile_row0 < g.M) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int64_t col0 = colbase + unit_of(i) * 16;
+                        const uint32_t* q = packed + i * 8;
+                        if (col0 < g.N) emit(make_uint4(q[0], q[1], q[2], q[3]), make_uint4(q[4], q[5], q[6], q[7]), row, col0, tile_row0);
+                    }
+                }
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < 8; ++i) {
+                    uint32_t r[16];
+                    read(i, r);
+                    const int64_t col0 = colbase + unit_of(i) * 16;
+                    if (tile_row0 < g.M && col0 < g.N) emit(make_uint4(r[0], r[1], r[2], r[3]), make_uint4(r[4], r[5], r[6], r[7]), row, col0, tile_row0);
+                    if (tile_row0 < g.M && col0 + 8 < g.N)
+                        emit(make_uint4(r[8], r[9], r[10], r[11]), make_uint4(r[12], r[13], r[14], r[15]), row, col0 + 8, tile_row0);
+                }
+            }
+        }
+        if (lane == 0) bulk_wait_all();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();      // neither CTA leaves while the other may still touch its memory or barriers
+    if (threadIdx.x == 0 && *abort_flag && g.status) atomicExch(g.status, NVFP4_ERR_TIMEOUT);
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "n"(TMEM_COLS) : "memory");
+    }
+}
+
+// ====================================================================================================================
+// one 128 x 128 tile per cluster, the contraction split over its CTAs
+// ====================================================================================================================
+namespace split8 {
+constexpr int THREADS = 192, STAGES = 6;
+constexpr int OPERANDS = 2 * G8_OPERAND, SCALES = 2 * G8_SF, STAGE_BYTES = OPERANDS + SCALES;
+constexpr int SF_BASE = 128, SF_COLS = 8, TMEM_COLS = 256;
+constexpr int PITCH = 132;                           // floats per row of the partial tile: lanes of a quarter warp hit different banks
+constexpr int BARS = 2 * STAGES + 1;
+constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256;
+static_assert(128 * PITCH * 4 <= STAGES * OPERANDS && BARS * 8 + 16 <= 256 && SMEM <= 232448, "budgets");
+}  // namespace split8
+
+__device__ __forceinline__ float4 cluster_load4(uint32_t addr, int rank) {     // 16 bytes at this shared-memory offset of CTA `rank`
+    uint32_t there;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(there) : "memory");
+    return v;
+}
+
+template <typename TO>
+__global__ void __launch_bounds__(split8::THREADS, 1)
+fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_sfa,
+                      const __grid_constant__ CUtensorMap map_sfb, const Gemm8Args g, const int splits) {
+    using namespace split8;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sf_smem = smem + STAGES * OPERANDS;
+    uint64_t* full = reinterpret_cast<uint64_t*>(sf_smem + STAGES * SCALES);
+    uint64_t* empty = full + STAGES;
+    uint64_t* acc_full = empty + STAGES;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const int rank = splits > 1 ? static_cast<int>(cluster_rank()) : 0;
+    const int tile = static_cast<int>(blockIdx.x) / splits;
+    const int tm = tile % g.tiles_m, tn = tile / g.tiles_m;
+    const int k0 = static_cast<int>(static_cast<int64_t>(g.k_tiles) * rank / splits), k1 = static_cast<int>(static_cast<int64_t>(g.k_tiles) * (rank + 1) / splits);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        mbar_init(acc_full, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0) {
+        bool ok = true;
+        int kt = k0;
+        for (int i = 0; kt < k1; ++kt, ++i) {
+            const int stage = i % STAGES;
+            if (!mbar_wait_warp(&empty[stage], ((i / STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
+            if (elect_one()) {
+                uint8_t* st = smem + stage * OPERANDS;
+                uint8_t* sf = sf_smem + stage * SCALES;
+                mbar_expect_tx(&full[stage], STAGE_BYTES);
+                tma_load_2d(st + G8_OPERAND, &map_b, kt * G8_BK, tn * 128, &full[stage]);
+                tma_load_2d(st, &map_a, kt * G8_BK, tm * 128, &full[stage]);
+                tma_load_2d(sf, &map_sfa, 0, tm * g.k_tiles + kt, &full[stage]);
+                tma_load_2d(sf + G8_SF, &map_sfb, 0, tn * g.k_tiles + kt, &full[stage]);
+            }
+            __syncwarp();
+        }
+        if (!ok && lane == 0) {      // a bounded chance for the loads in flight to land
+            for (int i = max(0, kt - k0 - STAGES); i < kt - k0; ++i) {
+                const long long t0 = clock64();
+                while (!mbar_try(&full[i % STAGES], (i / STAGES) & 1) && clock64() - t0 < WAIT_CYCLES / 8) {}
+            }
+        }
+    } else if (warp == 1) {
+        const uint32_t idesc = instr_desc8(128, 128);
+        bool ok = true;
+        for (int i = 0; i < k1 - k0; ++i) {
+            const int stage = i % STAGES;
+            if (!mbar_wait_warp(&full[stage], (i / STAGES) & 1, abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            if (elect_one()) {
+                const uint32_t sa = smem_u32(smem + stage * OPERANDS), sb = sa + G8_OPERAND, sf = smem_u32(sf_smem + stage * SCALES);
+                const uint32_t tsfa = tmem_base + SF_BASE + (i & 1) * SF_COLS, tsfb = tsfa + 4;
+                tc_cp_sf(tsfa, scale_desc(sf));
+                tc_cp_sf(tsfb, scale_desc(sf + G8_SF));
+#pragma unroll
+                for (int kb = 0; kb < 4; ++kb)
+                    mma8<false>(tmem_base, operand_desc(sa + kb * 32), operand_desc(sb + kb * 32), idesc, (i | kb) ? 1u : 0u, tsfa, tsfb);
+                tc_commit(&empty[stage]);
+            }
+            __syncwarp();
+        }
+        if (ok && elect_one()) tc_commit(acc_full);
+        __syncwarp();
+    } else if (mbar_wait_warp(acc_full, 0, abort_flag)) {
+        // every MMA has read its operands: their shared memory takes the FP32 partial tile, one row per lane
+        tc_fence_after();
+        const int row = (warp & 3) * 32 + lane;
+        const uint32_t taddr = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        float* mine = reinterpret_cast<float*>(smem) + row * PITCH;
+        const bool live = tm * 128 + row < g.M;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            uint32_t r[16];
+            tc_ld16(taddr + u * 16, r);
+            tc_wait_ld();
+            if (live) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    *reinterpret_cast<uint4*>(mine + u * 16 + j * 4) = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (splits > 1) cluster_sync();
+    if (!*abort_flag) {
+        // groups of four columns of the live rows, shared out over the cluster; the partial sums are added in rank order
+        const int rows = min(128, g.M - tm * 128);
+        const int64_t col_tile = static_cast<int64_t>(tn) * 128;
+        const uint32_t base = smem_u32(smem);
+        for (int e = rank * THREADS + threadIdx.x; e < rows * 32; e += splits * THREADS) {
+            const int r = e >> 5, c = (e & 31) * 4;
+            const uint32_t at = base + (r * PITCH + c) * 4;
+            const int64_t col = col_tile + c;
+            if (col >= g.N) continue;
+            float f[4];
+            if (splits > 1) {
+                float4 v = cluster_load4(at, 0);
+                for (int s = 1; s < splits; ++s) {
+                    const float4 w = cluster_load4(at, s);
+                    v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+                }
+                f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+            } else {
+                const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem) + r * PITCH + c);
+                f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+            }
+            TO* dst = static_cast<TO*>(g.out) + (static_cast<int64_t>(tm) * 128 + r) * g.ldo + col;
+            if (g.bias) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (col + j < g.N) f[j] += bias_at(g, col + j);
+            }
+            if (col + 4 <= g.N && (reinterpret_cast<uintptr_t>(dst) & (4 * sizeof(TO) - 1)) == 0) {
+                store_pack(dst, pack<TO, 4>(f));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (col + j < g.N) dst[j] = from_float<TO>(f[j]);
+            }
+        }
+    }
+    __syncthreads();
+    if (splits > 1) cluster_sync();      // a CTA's partial tile stays until the others have read it
+    if (threadIdx.x == 0 && *abort_flag && g.status) atomicExch(g.status, NVFP4_ERR_TIMEOUT);
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "n"(TMEM_COLS) : "memory");
+    }
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------
+static bool map_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t inner, int64_t outer, int64_t pitch_bytes, int box_inner,
+                   int box_outer, CUtensorMapSwizzle swizzle) {
+    aop::EncodeTiledFn fn = aop::encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
+    cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch_bytes)};
+    cuuint32_t box[2] = {static_cast<cuuint32_t>(box_inner), static_cast<cuuint32_t>(box_outer)};
+    cuuint32_t one[2] = {1, 1};
+    return fn(map, type, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+static bool operand_map(CUtensorMap* map, const uint8_t* base, int64_t rows, int64_t k) {
+    return map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, k, rows, k, G8_BK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+static bool scale_map(CUtensorMap* map, const uint8_t* base, int64_t rows, int64_t k) {      // one 512-byte block per row
+    return map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, G8_SF / 4, (rows + 127) / 128 * (k / 128), G8_SF, G8_SF / 4, 1, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+// 0: paired CTAs on 256 x 256 tiles; else the number of CTAs that share a 128 x 128 tile's contraction.  Estimated cycles: a
+// stage of the paired kernel takes 512 (its four instructions at the tensor cores' rate), one of the split kernel about 300
+// (256 of tensor time, plus its operands' shared-memory reads, which N = 128 instructions do not hide); a tile costs about
+// 1500 more for filling the pipeline and draining it, joining partial tiles another 1500.
+static int split_for(const Gemm8Args& g, int sms) {
+    auto waves = [](int64_t work, int64_t slots) { return (work + slots - 1) / slots; };
+    int64_t best = waves(static_cast<int64_t>((g.M + 255) / 256) * ((g.N + 255) / 256), sms / 2) * (g.k_tiles * 512LL + 1500);
+    int pick = 0;
+    const int64_t tiles = static_cast<int64_t>((g.M + 127) / 128) * ((g.N + 127) / 128);
+    for (int s = 1; s <= 8 && s <= g.k_tiles; s *= 2) {
+        const int64_t cost = waves(tiles * s, sms) * (waves(g.k_tiles, s) * 300LL + 1500) + (s > 1 ? 1500 : 0);
+        if (cost < best) { best = cost; pick = s; }
+    }
+    return pick;
+}
+
+template <typename TO>
+static int launch_gemm8(Gemm8Args& g, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& msa, const CUtensorMap& msb, cudaStream_t st) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    static bool configured[64] = {};
+    static int sm_count[64] = {};
+    NVFP4_REQUIRE(dev >= 0 && dev < 64, NVFP4_ERR_UNSUPPORTED, "nvfp4_fp8_gemm: device index above 63");
+    if (!configured[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(fp8_gemm_kernel<TO>, cudaFuncAttributeMaxDynamicSharedMemorySize, pair8::SMEM);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_gemm_split_kernel<TO>, cudaFuncAttributeMaxDynamicSharedMemorySize, split8::SMEM);
+        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sm_count[dev], cudaDevAttrMultiProcessorCount, dev);
+        NVFP4_REQUIRE(e == cudaSuccess, NVFP4_ERR_LAUNCH, "nvfp4_fp8_gemm: cannot configure the kernels: %s", cudaGetErrorString(e));
+        configured[dev] = true;
+    }
+    const int splits = split_for(g, sm_count[dev]);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e;
+    if (splits == 0) {
+        CUtensorMap mo = ma;           // unused without tma_store, but the parameter must hold a valid map
+        constexpr int ESZ = sizeof(TO);
+        g.tiles_m = (g.M + 255) / 256;
+        g.tiles_n = (g.N + 255) / 256;
+        g.tma_store = aligned(g.out, 16) && g.ldo * ESZ % 16 == 0 &&
+                      map_2d(&mo, ESZ == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, g.out, g.N, g.M, g.ldo * ESZ, 32 / ESZ, 32,
+                             CU_TENSOR_MAP_SWIZZLE_32B);
+        attr[0].val.clusterDim.x = 2;
+        cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min<int64_t>(static_cast<int64_t>(g.tiles_m) * g.tiles_n, sm_count[dev] / 2)));
+        cfg.blockDim = dim3(pair8::THREADS);
+        cfg.dynamicSmemBytes = pair8::SMEM;
+        e = cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<TO>, ma, mb, msa, msb, mo, g);
+    } else {
+        g.tiles_m = (g.M + 127) / 128;
+        g.tiles_n = (g.N + 127) / 128;
+        attr[0].val.clusterDim.x = splits;
+        cfg.gridDim = dim3(static_cast<unsigned>(g.tiles_m * g.tiles_n * splits));
+        cfg.blockDim = dim3(split8::THREADS);
+        cfg.dynamicSmemBytes = split8::SMEM;
+        e = cudaLaunchKernelEx(&cfg, fp8_gemm_split_kernel<TO>, ma, mb, msa, msb, g, splits);
+    }
+    NVFP4_REQUIRE(e == cudaSuccess, NVFP4_ERR_LAUNCH, "nvfp4_fp8_gemm: cluster launch failed: %s", cudaGetErrorString(e));
+    return launch_status("nvfp4_fp8_gemm");
+}
+
+}  // namespace nvfp4
+
+using namespace nvfp4;
+
+extern "C" int nvfp4_fp8_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* b, const uint8_t* b_scales, int64_t M, int64_t N, int64_t K,
+                              const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo, int* status, nvfp4_stream_t stream) {
+    NVFP4_REQUIRE(a && a_scales && b && b_scales && out, NVFP4_ERR_ARG, "nvfp4_fp8_gemm: null pointer");
+    NVFP4_REQUIRE(M > 0 && N > 0 && K > 0 && K % 128 == 0 && ldo >= N, NVFP4_ERR_ARG,
+                  "nvfp4_fp8_gemm: M, N and K must be positive, K a multiple of 128, ldo at least N (got %lld %lld %lld %lld)", (long long)M, (long long)N,
+                  (long long)K, (long long)ldo);
+    // tile coordinates and scale-block indices are 32-bit
+    NVFP4_REQUIRE(M < (1LL << 30) && N < (1LL << 30) && K < (1LL << 30) && ((M + 255) / 128 + 1) * (K / 128) < (1LL << 31) &&
+                  ((N + 255) / 128 + 1) * (K / 128) < (1LL << 31) && ((M + 127) / 128) * ((N + 127) / 128) < (1LL << 27), NVFP4_ERR_ARG,
+                  "nvfp4_fp8_gemm: sizes exceed the tile index range");
+    NVFP4_REQUIRE(is_float_dtype(out_dtype) && (!bias || is_float_dtype(bias_dtype)), NVFP4_ERR_DTYPE, "nvfp4_fp8_gemm: FP32, BF16 or FP16 result and bias");
+    for (const void* p : {static_cast<const void*>(a), static_cast<const void*>(a_scales), static_cast<const void*>(b), static_cast<const void*>(b_scales)})
+        NVFP4_REQUIRE(aligned(p, 16), NVFP4_ERR_ALIGN, "nvfp4_fp8_gemm: operands and scales must be 16-byte aligned");
+    NVFP4_REQUIRE(aligned(out, dtype_size(out_dtype)) && aligned(bias, bias ? dtype_size(bias_dtype) : 1), NVFP4_ERR_ALIGN,
+                  "nvfp4_fp8_gemm: result and bias must be aligned to their elements");
+    Gemm8Args g{bias, out, status, ldo, bias_dtype, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K / 128), 0, 0, 0};
+    CUtensorMap ma, mb, msa, msb;
+    NVFP4_REQUIRE(operand_map(&ma, a, M, K) && operand_map(&mb, b, N, K) && scale_map(&msa, a_scales, M, K) && scale_map(&msb, b_scales, N, K),
+                  NVFP4_ERR_LAUNCH, "nvfp4_fp8_gemm: cuTensorMapEncodeTiled failed or is unavailable");
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (out_dtype == NVFP4_BF16) return launch_gemm8<__nv_bfloat16>(g, ma, mb, msa, msb, st);
+    if (out_dtype == NVFP4_F16) return launch_gemm8<__half>(g, ma, mb, msa, msb, st);
+    return launch_gemm8<float>(g, ma, mb, msa, msb, st);
+}

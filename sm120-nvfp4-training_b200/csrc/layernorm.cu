@@ -509,3 +509,11 @@ extern "C" int nvfp4_layer_norm_bwd(const void* dh, int h_dtype, int64_t dh_pitc
         column_sums_kernel<<<static_cast<unsigned>((2 * cols + 31) / 32), 256, 0, st>>>(partial, parts, 2 * cols, cols, dweight, dbias, weight_dtype);
     return launch_status("nvfp4_layer_norm_bwd");
 }
+
+extern "C" int nvfp4_column_sums(const float* partial, int64_t parts, int64_t cols, void* out, int out_dtype, nvfp4_stream_t stream) {
+    NVFP4_REQUIRE(partial && out && parts > 0 && cols > 0 && cols < (1LL << 31), NVFP4_ERR_ARG, "nvfp4_column_sums: null pointer or empty size");
+    NVFP4_REQUIRE(is_float_dtype(out_dtype), NVFP4_ERR_DTYPE, "nvfp4_column_sums: FP32, BF16 or FP16 result");
+    column_sums_kernel<<<static_cast<unsigned>((cols + 31) / 32), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+        partial, parts, cols, cols, out, nullptr, out_dtype);
+    return launch_status("nvfp4_column_sums");
+}

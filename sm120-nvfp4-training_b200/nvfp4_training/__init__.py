@@ -9,10 +9,12 @@ from ._runtime import load_runtime
 __all__ = ["list_profiles", "prepare_training", "enable_nvfp4", "train_step", "capture_step", "save_checkpoint", "load_checkpoint",
            "check_finite", "enable_lora", "prepare_lora", "lora_parameters", "save_lora", "load_lora", "merge_lora",
            "capture_lora_step", "PackedNVFP4Linear", "pack_frozen_layers", "save_frozen_cache", "load_frozen_cache", "capture_frozen",
-           "enable_data_parallel", "layer_norm", "add_layer_norm", "LayerNorm", "rotary_axes", "rotary_axes_qkv"]
+           "enable_data_parallel", "layer_norm", "add_layer_norm", "LayerNorm", "rotary_axes", "rotary_axes_qkv",
+           "fp8_linear", "fp8_pack", "PackedFP8", "FP8Linear"]
 
 _LORA = {"enable_lora", "prepare_lora", "lora_parameters", "save_lora", "load_lora", "merge_lora", "PackedNVFP4Linear", "capture_lora_step"}
 _OPERATORS = {"layer_norm", "add_layer_norm", "LayerNorm", "rotary_axes", "rotary_axes_qkv"}
+_FP8 = {"fp8_linear", "fp8_pack", "PackedFP8", "FP8Linear"}
 
 
 def __getattr__(name):
@@ -20,9 +22,9 @@ def __getattr__(name):
     if name in _LORA:
         from . import lora
         return getattr(lora, name)
-    if name in _OPERATORS:
-        from . import operators
-        globals()[name] = getattr(operators, name)
+    if name in _OPERATORS or name in _FP8:
+        from . import fp8, operators
+        globals()[name] = getattr(fp8 if name in _FP8 else operators, name)
         return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 

@@ -99,3 +99,58 @@ def test_entry_points_refuse_before_any_launch():
     assert rotary(address=C.addressof(buf) + 1) == 2
     axis[3] = 1
     assert rotary() == 1 and b"axis" in lib.nvfp4_last_error()
+
+
+W = x(6, 16)
+
+
+@pytest.mark.parametrize("error,call", [
+    (TypeError, lambda: nv.fp8_linear(x(2, 16, dtype=torch.float64), W)),
+    (TypeError, lambda: nv.fp8_linear(x(2, 16), W.to(torch.float8_e4m3fn))),
+    (TypeError, lambda: nv.fp8_linear(x(2, 16), None)),
+    (ValueError, lambda: nv.fp8_linear(x(2, 15), W)),
+    (ValueError, lambda: nv.fp8_linear(x(), W)),
+    (ValueError, lambda: nv.fp8_linear(x(2, 16), x(16))),
+    (ValueError, lambda: nv.fp8_linear(x(2, 0), x(6, 0))),
+    (ValueError, lambda: nv.fp8_linear(x(2, 16), x(0, 16))),
+    (ValueError, lambda: nv.fp8_linear(x(2, 16), W, x(5))),
+    (ValueError, lambda: nv.fp8_linear(x(2, 16), W, x(12)[::2])),
+    (TypeError, lambda: nv.fp8_linear(x(2, 16), W, x(6, dtype=torch.int8))),
+    (ValueError, lambda: nv.fp8_linear(x(2, 16), W)),                                 # CPU tensors
+    (TypeError, lambda: nv.fp8_pack(x(6, 16, dtype=torch.uint8))),
+    (ValueError, lambda: nv.fp8_pack(x(6))),
+    (ValueError, lambda: nv.fp8_pack(x(6, 0))),
+    (ValueError, lambda: nv.fp8_pack(W)),
+])
+def test_fp8_refusals(error, call):
+    with pytest.raises(error):
+        call()
+
+
+def test_packed_weight_without_its_transpose_refuses_input_gradients():
+    packed = nv.PackedFP8(torch.zeros(6, 128, dtype=torch.uint8), torch.full((512,), 127, dtype=torch.uint8), None, None, (6, 16), BF16)
+    assert packed.dequantize().shape == (6, 16)
+    with pytest.raises(ValueError, match="transpose"):
+        nv.fp8_linear(x(2, 16).requires_grad_(True), packed)
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+        nv.fp8_linear(x(2, 16).requires_grad_(True), packed)
+
+
+def test_fp8_entry_points_refuse_before_any_launch():
+    from nvfp4_training import _native
+    lib = _native.lib()
+    buf = C.create_string_buffer(4096 + 16)
+    at = (C.addressof(buf) + 15) // 16 * 16
+
+    def quantize(x=at, dt=1, rows=4, cols=8, pitch=8, codes=at, scales=at, codes_t=None, scales_t=None, sums=None):
+        return lib.nvfp4_fp8_quantize(x, dt, rows, cols, pitch, 0, codes, scales, codes_t, scales_t, sums, None)
+    assert quantize(x=None) == 1 and quantize(codes=None, scales=None) == 1 and quantize(scales=None) == 1 and quantize(codes_t=at) == 1
+    assert quantize(rows=0) == 1 and quantize(cols=0) == 1 and quantize(pitch=7) == 1 and quantize(sums=at) == 1
+    assert quantize(dt=3) == 3 and quantize(codes=at + 1) == 2
+
+    def gemm(a=at, m=4, n=8, k=128, bias=None, bd=0, out=at, od=1, ldo=8):
+        return lib.nvfp4_fp8_gemm(a, at, at, at, m, n, k, bias, bd, out, od, ldo, None, None)
+    assert gemm(a=None) == 1 and gemm(out=None) == 1 and gemm(m=0) == 1 and gemm(n=0) == 1 and gemm(k=64) == 1 and gemm(ldo=7) == 1
+    assert gemm(k=0) == 1 and gemm(m=1 << 30) == 1 and gemm(m=1 << 29, n=1 << 29, ldo=1 << 29) == 1
+    assert gemm(od=3) == 3 and gemm(bias=at, bd=4) == 3 and gemm(a=at + 8) == 2 and gemm(out=at + 1) == 2
+    assert lib.nvfp4_column_sums(at, 0, 8, at, 0, None) == 1 and lib.nvfp4_column_sums(at, 1, 8, at, 3, None) == 3
