@@ -113,6 +113,28 @@ def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *_):
+        return False
+
+
+_HERE = _Here()
+
+
+def on(device: torch.device):
+    """torch.cuda.device(device) where that is another device than the current one, and nothing where it is this one: a
+    small call's launch is otherwise mostly this switch."""
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+def raw_stream(device: torch.device) -> int:
+    """Handle of the device's current stream (stream_of without the Stream object)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 _SCRATCH: dict[tuple, torch.Tensor] = {}
 
 

@@ -16,7 +16,7 @@ import torch
 from torch import nn
 
 from . import _native as nat
-from .operators import _check_device, _check_tensor
+from .operators import _check_device, _check_tensor, pitch_of, rows_of
 
 _MAX = 1 << 30
 
@@ -52,51 +52,59 @@ def _quantize(x, *, row, col, square=False, column_sums=False):
     """((codes, scales) or None, (codes_t, scales_t) or None, FP32 partial column sums or None) of x [rows, cols]."""
     rows, cols = x.shape
     rb, cb = _ceil128(rows), _ceil128(cols)
-    new = lambda *shape: torch.empty(shape, dtype=torch.uint8, device=x.device)
-    a = (new(rows, cb * 128), new(rb * cb * 512)) if row else (None, None)
-    t = (new(cols, rb * 128), new(cb * rb * 512)) if col else (None, None)
-    sums = torch.empty((rb, cols), dtype=torch.float32, device=x.device) if column_sums else None
-    with torch.cuda.device(x.device):
-        nat.check(nat.lib().nvfp4_fp8_quantize(x.data_ptr(), nat.dtype_code(x), rows, cols, max(x.stride(0), cols), int(square), nat.ptr(a[0]),
-                                               nat.ptr(a[1]), nat.ptr(t[0]), nat.ptr(t[1]), nat.ptr(sums), nat.stream_of(x)))
+    dev = x.device
+    a, t, sums = (None, None), (None, None), None
+    if row:
+        a = (torch.empty((rows, cb * 128), dtype=torch.uint8, device=dev), torch.empty(rb * cb * 512, dtype=torch.uint8, device=dev))
+    if col:
+        t = (torch.empty((cols, rb * 128), dtype=torch.uint8, device=dev), torch.empty(cb * rb * 512, dtype=torch.uint8, device=dev))
+    if column_sums:
+        sums = torch.empty((rb, cols), dtype=torch.float32, device=dev)
+    with nat.on(dev):
+        nat.check(nat.lib().nvfp4_fp8_quantize(x.data_ptr(), nat._CODES[x.dtype], rows, cols, pitch_of(x), square, nat.ptr(a[0]), nat.ptr(a[1]),
+                                               nat.ptr(t[0]), nat.ptr(t[1]), nat.ptr(sums), nat.raw_stream(dev)))
     return (a if row else None), (t if col else None), sums
 
 
 def _gemm(a, b, k, dtype, bias=None, out=None):
     """a, b: (codes, scales) of [M, k] and [N, k]."""
     m, n = a[0].shape[0], b[0].shape[0]
+    dev = a[0].device
     if out is None:
-        out = torch.empty((m, n), dtype=dtype, device=a[0].device)
-    with torch.cuda.device(out.device):
+        out = torch.empty((m, n), dtype=dtype, device=dev)
+    with nat.on(dev):
         nat.check(nat.lib().nvfp4_fp8_gemm(a[0].data_ptr(), a[1].data_ptr(), b[0].data_ptr(), b[1].data_ptr(), m, n, _ceil128(k) * 128, nat.ptr(bias),
-                                           0 if bias is None else nat.dtype_code(bias), out.data_ptr(), nat.dtype_code(out), out.stride(0),
-                                           nat.status_word(out.device).data_ptr(), nat.stream_of(out)))
+                                           0 if bias is None else nat._CODES[bias.dtype], out.data_ptr(), nat._CODES[out.dtype], out.stride(0),
+                                           nat.status_word(dev).data_ptr(), nat.raw_stream(dev)))
     return out
 
 
 def _column_sums(partial, dtype):
     out = torch.empty(partial.shape[1], dtype=dtype, device=partial.device)
-    with torch.cuda.device(out.device):
-        nat.check(nat.lib().nvfp4_column_sums(partial.data_ptr(), partial.shape[0], partial.shape[1], out.data_ptr(), nat.dtype_code(out), nat.stream_of(out)))
+    with nat.on(out.device):
+        nat.check(nat.lib().nvfp4_column_sums(partial.data_ptr(), partial.shape[0], partial.shape[1], out.data_ptr(), nat._CODES[dtype],
+                                              nat.raw_stream(out.device)))
     return out
 
 
-def _flat(t, cols):
-    """[rows, cols] with contiguous rows (any row pitch); a copy only where the layout has no such view."""
-    flat = t.reshape(-1, cols)
-    if (cols > 1 and flat.stride(1) != 1) or (flat.shape[0] > 1 and flat.stride(0) < cols):
-        flat = flat.contiguous()
-    return flat
+def _inference(x, weight, bias, packed):
+    n, k = packed.shape if weight is None else weight.shape
+    x2 = rows_of(x, k)
+    if not x2.shape[0]:
+        return torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
+    wq = (packed.codes, packed.scales) if weight is None else _quantize(rows_of(weight, k), row=True, col=False, square=True)[0]
+    y = _gemm(_quantize(x2, row=True, col=False)[0], wq, k, x.dtype, bias)
+    return y if x.ndim == 2 else y.view(*x.shape[:-1], n)
 
 
 class _Fp8Linear(torch.autograd.Function):
     """weight: the parameter [N, K], packed on every call, or None beside a packed one."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, packed, active):
-        need_x, need_w, need_b = (active and need for need in ctx.needs_input_grad[:3])
+    def forward(ctx, x, weight, bias, packed):
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
         n, k = packed.shape if weight is None else weight.shape
-        x2 = _flat(x, k)
+        x2 = rows_of(x, k)
         m = x2.shape[0]
         ctx.dims, ctx.need, ctx.shape, ctx.dtype = (m, k, n), (need_x, need_w, need_b), x.shape, x.dtype
         ctx.bias_dtype, ctx.weight_dtype = None if bias is None else bias.dtype, None if weight is None else weight.dtype
@@ -107,7 +115,7 @@ class _Fp8Linear(torch.autograd.Function):
         if weight is None:
             wq, wt = (packed.codes, packed.scales), (packed.codes_t, packed.scales_t)
         else:
-            wq, wt, _ = _quantize(_flat(weight.detach(), k), row=True, col=need_x, square=True)
+            wq, wt, _ = _quantize(rows_of(weight.detach(), k), row=True, col=need_x, square=True)
         y = _gemm(xq, wq, k, x.dtype, bias)
         ctx.save_for_backward(weight, *(wt if need_x else (None, None)), *(xt if need_w else (None, None)))
         return y.view(*x.shape[:-1], n)
@@ -120,17 +128,17 @@ class _Fp8Linear(torch.autograd.Function):
         weight = ctx.saved_tensors[0]
         if m == 0:
             zero = lambda yes, shape, dtype: torch.zeros(shape, dtype=dtype, device=grad.device) if yes else None
-            return zero(need_x, ctx.shape, ctx.dtype), zero(need_w, (n, k), ctx.weight_dtype), zero(need_b, (n,), ctx.bias_dtype), None, None
+            return zero(need_x, ctx.shape, ctx.dtype), zero(need_w, (n, k), ctx.weight_dtype), zero(need_b, (n,), ctx.bias_dtype), None
         _, wt_codes, wt_scales, xt_codes, xt_scales = ctx.saved_tensors
         dx = dw = db = None
-        gq, gt, sums = _quantize(_flat(grad, n), row=need_x, col=need_w or need_b, column_sums=need_b)
+        gq, gt, sums = _quantize(rows_of(grad, n), row=need_x, col=need_w or need_b, column_sums=need_b)
         if need_x:
             dx = _gemm(gq, (wt_codes, wt_scales), n, ctx.dtype).view(ctx.shape)
         if need_w:
             dw = _weight_gradient(weight, gt, (xt_codes, xt_scales), m)
         if need_b:
             db = _column_sums(sums, ctx.bias_dtype)
-        return dx, dw, db, None, None
+        return dx, dw, db, None
 
 
 def _weight_gradient(weight, gt, xt, tokens):
@@ -160,7 +168,7 @@ def fp8_pack(weight, *, transpose=True):
     if weight.ndim != 2 or 0 in weight.shape or max(weight.shape) >= _MAX:
         raise ValueError("weight must be [out_features, in_features], not empty")
     _check_device(weight)
-    w = _flat(weight.detach(), weight.shape[1])
+    w = rows_of(weight.detach(), weight.shape[1])
     q, t, _ = _quantize(w, row=True, col=transpose, square=True)
     return PackedFP8(*q, *(t if transpose else (None, None)), tuple(weight.shape), weight.dtype)
 
@@ -187,7 +195,11 @@ def fp8_linear(x, weight, bias=None):
     if packed is not None and packed.codes_t is None and x.requires_grad and torch.is_grad_enabled():
         raise ValueError("This weight was packed without its transpose: no gradient can reach x")
     _check_device(x)
-    return _Fp8Linear.apply(x, None if packed is not None else weight, bias, packed, torch.is_grad_enabled())
+    if packed is not None:
+        weight = None
+    if not (torch.is_grad_enabled() and (x.requires_grad or any(t is not None and t.requires_grad for t in (weight, bias)))):
+        return _inference(x, weight, bias, packed)
+    return _Fp8Linear.apply(x, weight, bias, packed)
 
 
 class FP8Linear(nn.Linear):

@@ -36,46 +36,58 @@ def _zeroed_slot(device):
 
 
 # ---- layer norm -------------------------------------------------------------------------------------------------------
-def _rows(t, cols):
+def rows_of(t, cols):
     """[rows, cols] view with contiguous rows (any row pitch); a copy only where the layout has no such view."""
+    if t.ndim == 2 and t.is_contiguous():
+        return t
     flat = t.reshape(-1, cols)
     if (cols > 1 and flat.stride(1) != 1) or (flat.shape[0] > 1 and flat.stride(0) < cols):
         flat = flat.contiguous()
     return flat
 
 
-def _pitch(flat):
+def pitch_of(flat):
     return max(flat.stride(0), flat.shape[1])
+
+
+def _norm_forward(x, delta, weight, bias, eps, out_dtype, amax, keep_stats):
+    """(total [rows, cols], h, statistics or None): h and a new total in x's shape, total as rows."""
+    shape, dev = x.shape, x.device
+    cols = shape[-1]
+    x2 = rows_of(x, cols)
+    rows = x2.shape[0]
+    d2, total = None, x2
+    if delta is not None:
+        d2 = rows_of(delta, cols)
+        total = torch.empty((rows, cols), dtype=x.dtype, device=dev)
+    h = torch.empty(shape, dtype=out_dtype, device=dev)
+    stats = torch.empty(2 * rows, dtype=torch.float32, device=dev) if keep_stats else None
+    if rows:
+        at = stats.data_ptr() if keep_stats else None
+        affine = weight if weight is not None else bias
+        codes = nat._CODES
+        with nat.on(dev):
+            nat.check(nat.lib().nvfp4_layer_norm(
+                x2.data_ptr(), codes[x.dtype], pitch_of(x2), nat.ptr(d2), 0 if d2 is None else codes[d2.dtype], 0 if d2 is None else pitch_of(d2),
+                nat.ptr(weight), nat.ptr(bias), 0 if affine is None else codes[affine.dtype], eps, rows, cols,
+                None if d2 is None else total.data_ptr(), h.data_ptr(), codes[out_dtype], at, at and at + 4 * rows, nat.ptr(amax), nat.raw_stream(dev)))
+    return total, h, stats
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, delta, weight, bias, eps, out_dtype, want_amax):
-        shape, cols, dev = x.shape, x.shape[-1], x.device
-        x2 = _rows(x, cols)
-        d2 = None if delta is None else _rows(delta, cols)
-        rows = x2.shape[0]
-        total = x2 if d2 is None else torch.empty((rows, cols), dtype=x.dtype, device=dev)
-        h = torch.empty((rows, cols), dtype=out_dtype, device=dev)
-        stats = torch.empty((2, rows), dtype=torch.float32, device=dev)
-        amax = _zeroed_slot(dev) if want_amax else None
-        affine = weight if weight is not None else bias
-        wcode = 0 if affine is None else nat.dtype_code(affine)
-        if rows:
-            with torch.cuda.device(dev):
-                nat.check(nat.lib().nvfp4_layer_norm(
-                    x2.data_ptr(), nat.dtype_code(x2), _pitch(x2), nat.ptr(d2), 0 if d2 is None else nat.dtype_code(d2),
-                    0 if d2 is None else _pitch(d2), nat.ptr(weight), nat.ptr(bias), wcode, eps, rows, cols,
-                    None if d2 is None else total.data_ptr(), h.data_ptr(), nat.dtype_code(h), stats[0].data_ptr(), stats[1].data_ptr(),
-                    nat.ptr(amax), nat.stream_of(x)))
+        amax = _zeroed_slot(x.device) if want_amax else None
+        total, h, stats = _norm_forward(x, delta, weight, bias, eps, out_dtype, amax, True)
         ctx.save_for_backward(total, stats, weight)
-        ctx.delta_dtype, ctx.shape, ctx.want_amax = None if delta is None else delta.dtype, shape, want_amax
+        affine = weight if weight is not None else bias
+        ctx.delta_dtype, ctx.shape, ctx.want_amax = None if delta is None else delta.dtype, x.shape, want_amax
         ctx.affine = (weight is not None and ctx.needs_input_grad[2], bias is not None and ctx.needs_input_grad[3],
                       None if affine is None else affine.dtype)
         ctx.set_materialize_grads(False)
         if amax is not None:
             ctx.mark_non_differentiable(amax)
-        return (None if d2 is None else total.view(shape)), h.view(shape), amax
+        return (None if delta is None else total.view(x.shape)), h, amax
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -88,30 +100,30 @@ class _LayerNorm(torch.autograd.Function):
             dd = None if (dsum is None or ctx.delta_dtype is None) else dsum.to(ctx.delta_dtype)
             zero = torch.zeros(cols, dtype=wdtype, device=dev) if (need_w or need_b) else None
             return dsum, dd, (zero if need_w else None), (zero if need_b else None), None, None, None
-        g = _rows(dh, cols)
-        res = None if dsum is None else _rows(dsum, cols)
-        dx = torch.empty((rows, cols), dtype=total.dtype, device=dev)
+        g = rows_of(dh, cols)
+        res = None if dsum is None else rows_of(dsum, cols)
+        dx = torch.empty(ctx.shape, dtype=total.dtype, device=dev)
         narrow = ctx.delta_dtype is not None and ctx.delta_dtype != total.dtype
-        dd = torch.empty((rows, cols), dtype=ctx.delta_dtype, device=dev) if narrow else None
+        dd = torch.empty(ctx.shape, dtype=ctx.delta_dtype, device=dev) if narrow else None
         dw = torch.empty(cols, dtype=wdtype, device=dev) if need_w else None
         db = torch.empty(cols, dtype=wdtype, device=dev) if need_b else None
         amax = _zeroed_slot(dev) if ctx.want_amax and (narrow or total.dtype == torch.bfloat16) else None
         if rows:
-            partial = None
+            lib, partial, codes = nat.lib(), None, nat._CODES
             if need_w or need_b:
-                parts = int(nat.lib().nvfp4_layer_norm_bwd_partials(rows, cols))
-                partial = torch.empty((parts, 2, cols), dtype=torch.float32, device=dev)
-            with torch.cuda.device(dev):
-                nat.check(nat.lib().nvfp4_layer_norm_bwd(
-                    g.data_ptr(), nat.dtype_code(g), _pitch(g), total.data_ptr(), nat.dtype_code(total), _pitch(total), stats[0].data_ptr(),
-                    stats[1].data_ptr(), nat.ptr(weight), 0 if wdtype is None else nat._CODES[wdtype], nat.ptr(res), 0 if res is None else _pitch(res),
-                    rows, cols, dx.data_ptr(), nat.ptr(dd), nat.ptr(partial), nat.ptr(dw), nat.ptr(db), nat.ptr(amax), nat.stream_of(total)))
+                partial = torch.empty(lib.nvfp4_layer_norm_bwd_partials(rows, cols) * 2 * cols, dtype=torch.float32, device=dev)
+            at = stats.data_ptr()
+            with nat.on(dev):
+                nat.check(lib.nvfp4_layer_norm_bwd(
+                    g.data_ptr(), codes[g.dtype], pitch_of(g), total.data_ptr(), codes[total.dtype], pitch_of(total), at, at + 4 * rows,
+                    nat.ptr(weight), 0 if wdtype is None else codes[wdtype], nat.ptr(res), 0 if res is None else pitch_of(res), rows, cols,
+                    dx.data_ptr(), nat.ptr(dd), nat.ptr(partial), nat.ptr(dw), nat.ptr(db), nat.ptr(amax), nat.raw_stream(dev)))
         else:
             for t in (dw, db):
                 if t is not None:
                     t.zero_()
-        dx = dx.view(ctx.shape)
-        dd = dd.view(ctx.shape) if narrow else (dx if ctx.delta_dtype is not None else None)
+        if not narrow and ctx.delta_dtype is not None:
+            dd = dx
         if amax is not None:
             attach_amax(dd if narrow else dx, amax)
         return dx, dd, dw, db, None, None, None
@@ -142,6 +154,10 @@ def _layer_norm(x, delta, weight, bias, eps, out_dtype, want_amax=False):
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError("weight and bias must have one dtype")
     _check_device(x)
+    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, delta, weight, bias))):
+        amax = _zeroed_slot(x.device) if want_amax and out_dtype == torch.bfloat16 else None
+        total, h, _ = _norm_forward(x, delta, weight, bias, eps, out_dtype, amax, False)
+        return (None if delta is None else total.view(x.shape)), h, amax
     return _LayerNorm.apply(x, delta, weight, bias, eps, out_dtype, want_amax and out_dtype == torch.bfloat16)
 
 
@@ -174,6 +190,7 @@ class LayerNorm(nn.LayerNorm):
 # ---- rotary positions over several axes -----------------------------------------------------------------------------------
 _POSITION_KINDS = {torch.int64: 0, torch.int32: 1, torch.float32: 2, torch.float64: 3}
 MAX_PAIRS = 256
+_Strides = C.c_int64 * 3
 
 
 class _Tensor(C.Structure):
@@ -196,47 +213,51 @@ def _plan(sections, theta, frequencies):
     return turns, axis, pairs
 
 
-def _launch_rotary(jobs, positions, plan, axes, dim, interleaved, inverse, amax):
+def _launch_rotary(jobs, positions, plan, axes, interleaved, inverse, amax):
     """jobs: (x, out, turn), each [batch, seq, heads, dim] with contiguous features."""
     x0 = jobs[0][0]
+    batch, seq, _, dim = x0.shape
     turns, axis, pairs = plan
-    tensors = (_Tensor * len(jobs))()
-    for t, (x, out, turn) in zip(tensors, jobs):
-        t.x, t.out, t.heads, t.turn = x.data_ptr(), out.data_ptr(), x.shape[2], int(turn)
-        t.x_stride[:], t.out_stride[:] = x.stride()[:3], out.stride()[:3]
-    ps = (0,) * (3 - positions.ndim) + positions.stride()
-    with torch.cuda.device(x0.device):
-        nat.check(nat.lib().nvfp4_rotary_axes(tensors, len(jobs), nat.dtype_code(x0), x0.shape[0], x0.shape[1], dim, positions.data_ptr(),
-                                              _POSITION_KINDS[positions.dtype], (C.c_int64 * 3)(*ps), axes, turns, axis, pairs,
-                                              int(interleaved), int(inverse), nat.ptr(amax), nat.stream_of(x0)))
+    tensors = (_Tensor * len(jobs))(*[(x.data_ptr(), out.data_ptr(), x.stride()[:3], out.stride()[:3], x.shape[2], turn) for x, out, turn in jobs])
+    ps = positions.stride() if positions.ndim == 3 else (0, *positions.stride())
+    dev = x0.device
+    with nat.on(dev):
+        nat.check(nat.lib().nvfp4_rotary_axes(tensors, len(jobs), nat._CODES[x0.dtype], batch, seq, dim, positions.data_ptr(),
+                                              _POSITION_KINDS[positions.dtype], _Strides(*ps), axes, turns, axis, pairs, interleaved, inverse,
+                                              nat.ptr(amax), nat.raw_stream(dev)))
 
 
 def _features_contiguous(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _turn(tensors, positions, how, inverse):
+    """Rotated copies of the tensors that are not None, in one launch."""
+    outs = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in tensors]
+    jobs = [(_features_contiguous(t), o, 1) for t, o in zip(tensors, outs) if t is not None and t.numel()]
+    if jobs:
+        _launch_rotary(jobs, positions, *how, inverse, None)
+    return outs
+
+
 class _RotaryAxes(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, positions, plan, axes, interleaved):
+    def forward(ctx, q, k, positions, how):
         ctx.save_for_backward(positions)
-        ctx.how = (plan, axes, interleaved)
+        ctx.how = how
         ctx.set_materialize_grads(False)
-        sources = [t for t in (q, k) if t is not None]
-        outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in sources]
-        if sources[0].numel():
-            _launch_rotary([(_features_contiguous(t), o, True) for t, o in zip(sources, outs)], positions, plan, axes, q.shape[3], interleaved, False, None)
-        return outs[0], (outs[1] if k is not None else None)
+        return tuple(_turn((q, k), positions, how, False))
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
         positions, = ctx.saved_tensors
-        plan, axes, interleaved = ctx.how
-        grads = [None if g is None else torch.empty(g.shape, dtype=g.dtype, device=g.device) for g in (dq, dk)]
-        jobs = [(_features_contiguous(g), o, True) for g, o in zip((dq, dk), grads) if g is not None and g.numel()]
-        if jobs:
-            _launch_rotary(jobs, positions, plan, axes, jobs[0][0].shape[3], interleaved, True, None)
-        return grads[0], grads[1], None, None, None, None
+        return (*_turn((dq, dk), positions, ctx.how, True), None, None)
+
+
+def _split_heads(t, heads, kv_heads):
+    b, s, width = t.shape
+    return t.view(b, s, heads + 2 * kv_heads, width // (heads + 2 * kv_heads)).split((heads, kv_heads, kv_heads), dim=2)
 
 
 class _RotaryFused(torch.autograd.Function):
@@ -244,37 +265,30 @@ class _RotaryFused(torch.autograd.Function):
     gradients together in one launch."""
 
     @staticmethod
-    def forward(ctx, qkv, positions, plan, axes, interleaved, heads, kv_heads):
-        b, s, width = qkv.shape
-        d = width // (heads + 2 * kv_heads)
+    def forward(ctx, qkv, positions, how, heads, kv_heads):
         ctx.save_for_backward(positions)
-        ctx.how, ctx.dims = (plan, axes, interleaved), (b, s, heads, kv_heads, d)
+        ctx.how, ctx.dims = how, (qkv.shape, heads, kv_heads)
         ctx.set_materialize_grads(False)
-        parts = qkv.detach().view(b, s, heads + 2 * kv_heads, d).split((heads, kv_heads, kv_heads), dim=2)
-        q = torch.empty((b, s, heads, d), dtype=qkv.dtype, device=qkv.device)
-        k = torch.empty((b, s, kv_heads, d), dtype=qkv.dtype, device=qkv.device)
-        if qkv.numel():
-            _launch_rotary([(parts[0], q, True), (parts[1], k, True)], positions, plan, axes, d, interleaved, False, None)
-        return q, k, parts[2]
+        q, k, v = _split_heads(qkv.detach(), heads, kv_heads)
+        return (*_turn((q, k), positions, how, False), v)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk, dv):
         positions, = ctx.saved_tensors
-        plan, axes, interleaved = ctx.how
-        b, s, heads, kv_heads, d = ctx.dims
+        shape, heads, kv_heads = ctx.dims
         some = next(g for g in (dq, dk, dv) if g is not None)
-        dqkv = torch.empty((b, s, (heads + 2 * kv_heads) * d), dtype=some.dtype, device=some.device)
+        dqkv = torch.empty(shape, dtype=some.dtype, device=some.device)
         amax = _zeroed_slot(some.device) if some.dtype == torch.bfloat16 else None
         jobs = []
-        for g, o, turn in zip((dq, dk, dv), dqkv.view(b, s, -1, d).split((heads, kv_heads, kv_heads), dim=2), (True, True, False)):
+        for g, o, turn in zip((dq, dk, dv), _split_heads(dqkv, heads, kv_heads), (1, 1, 0)):
             if g is None:
                 o.zero_()
             else:
                 jobs.append((_features_contiguous(g), o, turn))
         if dqkv.numel():
-            _launch_rotary(jobs, positions, plan, axes, d, interleaved, True, amax)
-        return (dqkv if amax is None else attach_amax(dqkv, amax)), None, None, None, None, None, None
+            _launch_rotary(jobs, positions, *ctx.how, True, amax)
+        return (dqkv if amax is None else attach_amax(dqkv, amax)), None, None, None, None
 
 
 def _check_rotary(x, batch, seq, dim, positions, sections, theta, layout, frequencies):
@@ -318,7 +332,9 @@ def rotary_axes(q, k, positions, sections, *, theta=10000.0, layout="half", freq
     if q.shape[2] == 0:
         raise ValueError("q needs at least one head")
     how = _check_rotary(q, q.shape[0], q.shape[1], q.shape[3], positions, sections, theta, layout, frequencies)
-    return _RotaryAxes.apply(q, k, positions, *how)
+    if not (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
+        return tuple(_turn((q, k), positions, how, False))
+    return _RotaryAxes.apply(q, k, positions, how)
 
 
 def rotary_axes_qkv(qkv, positions, sections, heads, kv_heads=None, *, theta=10000.0, layout="half", frequencies="shared"):
@@ -332,4 +348,8 @@ def rotary_axes_qkv(qkv, positions, sections, heads, kv_heads=None, *, theta=100
         raise ValueError("qkv must be [batch, seq, (heads + 2 * kv_heads) * dim]")
     dim = qkv.shape[2] // (heads + 2 * kv_heads)
     how = _check_rotary(qkv, qkv.shape[0], qkv.shape[1], dim, positions, sections, theta, layout, frequencies)
-    return _RotaryFused.apply(_features_contiguous(qkv), positions, *how, heads, kv_heads)
+    qkv = _features_contiguous(qkv)
+    if not (torch.is_grad_enabled() and qkv.requires_grad):
+        q, k, v = _split_heads(qkv, heads, kv_heads)
+        return (*_turn((q, k), positions, how, False), v)
+    return _RotaryFused.apply(qkv, positions, how, heads, kv_heads)
