@@ -59,10 +59,15 @@ def enable_data_parallel(model, process_group=None, *, bucket_mb=25.0, depth=2, 
 
 
 def prepare_training(model, *, profile="balanced", precision="fp4", remat=False, lr=1e-4, betas=(0.9, 0.999), eps=1e-8,
-                     weight_decay=0.01):
-    """Convert a fresh FP32 model in place and return (model, matching AdamW)."""
+                     weight_decay=0.01, fp8_layers=(), fused_norms=False):
+    """Convert a fresh FP32 model in place and return (model, matching AdamW).
+
+    fp8_layers: patterns of Linear layers (their path or an ancestor's, shell style) whose products run in 8 bits instead of
+    NVFP4, for layers that do not bear 4; masters and optimizer state keep the profile's format (not with the FP8-master
+    profile).  fused_norms: nn.LayerNorm modules over one dimension run on nvfp4_training.LayerNorm."""
     from ._convert import prepare
-    return prepare(model, profile=profile, precision=precision, remat=remat, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
+    return prepare(model, profile=profile, precision=precision, remat=remat, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
+                   fp8_layers=fp8_layers, fused_norms=fused_norms)
 
 
 def enable_nvfp4(model, *, profile="balanced", **options):

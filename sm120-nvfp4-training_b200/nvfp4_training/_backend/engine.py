@@ -16,6 +16,7 @@ import torch
 from torch import nn
 
 from .. import _native as nat
+from ..fp8 import FP8Linear
 from .linear import AutocastLinear, Linear6
 from .optimizer import FORMATS, AdamW, AdamW6, cdiv
 from .quant import get_signs
@@ -47,6 +48,7 @@ class _Plan:
     direct: bool
     remat: bool
     narrow: list          # Linear layers whose weight gets the format's narrow master
+    fp8: tuple = ()       # Linear layers whose products run in 8 bits instead of NVFP4
 
 
 def _check_request(model, mode, fmt, tiles, warps, mma_warps, prepack, remat, direct, compact_embedding):
@@ -113,6 +115,19 @@ def _attach_nvfp4(layer, remat):
         w._v6_remat = True
 
 
+def _attach_fp8(layer):
+    """8-bit products; the optimizer takes the weight's gradient from the layer, as it does from the NVFP4 layers."""
+    layer.__class__ = FP8Linear
+    layer.weight._v6_defer_dense = True
+
+
+def _check_fp8(layers, master, uses):
+    if layers and master == 8:
+        raise ValueError('8-bit layers read FP32, FP16 or BF16 masters; this storage format keeps E4M3 masters')
+    if any(uses[id(layer.weight)] != 1 for layer in layers):
+        raise ValueError('8-bit layers must own their weight: tied weights need one number format')
+
+
 def _narrow_on_device(layer, plan, opt):
     """The master storage of one layer (device conversion) and, for FP8, its checkpoint-visible unit vector."""
     p = layer.weight
@@ -130,10 +145,11 @@ def _narrow_on_device(layer, plan, opt):
 
 
 def configure(model, mode, fmt, *, lr=1e-4, tiles=4, warps=4, prepack=False, pack_warps=8, remat=False, direct=False, mma_k=0,
-              mma_warps=8, compact_embedding=False, act_pair=False, fast_scale=False):
+              mma_warps=8, compact_embedding=False, act_pair=False, fast_scale=False, fp8_layers=()):
     """Set up a fresh contiguous FP32 model (on CPU for direct conversion, else CUDA) for NVFP4 compute."""
     master = _check_request(model, mode, fmt, tiles, warps, mma_warps, prepack, remat, direct, compact_embedding)
-    plan = _Plan(master, direct, remat, _narrow_layers(model, master))
+    _check_fp8(fp8_layers, master, _uses(model))
+    plan = _Plan(master, direct, remat, _narrow_layers(model, master), tuple(fp8_layers))
     if master == 8:
         for layer in plan.narrow:
             unit = torch.tensor(unit_for(layer.weight), device=layer.weight.device, dtype=torch.float32)
@@ -146,7 +162,9 @@ def configure(model, mode, fmt, *, lr=1e-4, tiles=4, warps=4, prepack=False, pac
         _convert_on_host(model, plan)
     uses = _uses(model)
     for layer in model.modules():
-        if isinstance(layer, nn.Linear):
+        if any(layer is chosen for chosen in plan.fp8):
+            _attach_fp8(layer)
+        elif isinstance(layer, nn.Linear):
             _attach_nvfp4(layer, remat)
             p = layer.weight
             if uses[id(p)] == 1 and p.numel() >= NARROW_FROM and not remat:

@@ -10,6 +10,7 @@ import torch
 from torch import nn
 
 from ._runtime import load_runtime
+from .frozen import _matches
 from .profiles import profile_config
 
 
@@ -49,10 +50,33 @@ def _enforce(rules):
             raise error(message)
 
 
-def prepare(model, *, profile, precision, remat, lr, betas, eps, weight_decay):
+def _chosen(model, patterns):
+    """The Linear layers that the patterns name (by their path or an ancestor's, as in pack_frozen_layers)."""
+    if isinstance(patterns, str):
+        raise ValueError("Pass fp8_layers as a sequence of patterns, not a string")
+    layers = []
+    for pattern in patterns:
+        found = [m for name, m in model.named_modules() if isinstance(m, nn.Linear) and _matches(name, (pattern,))]
+        if not found:
+            raise ValueError(f"fp8_layers: {pattern!r} names no Linear layer")
+        layers.extend(m for m in found if not any(m is other for other in layers))
+    return tuple(layers)
+
+
+def _fuse_norms(model):
+    from .operators import LayerNorm
+    for module in model.modules():
+        if type(module) is nn.LayerNorm and len(module.normalized_shape) == 1:
+            module.__class__ = LayerNorm
+
+
+def prepare(model, *, profile, precision, remat, lr, betas, eps, weight_decay, fp8_layers=(), fused_norms=False):
     cfg = profile_config(profile)
     _enforce(_argument_rules(precision, remat, lr, betas, eps, weight_decay))
     _enforce(_model_rules(model))
+    fp8_layers = _chosen(model, fp8_layers)
+    if type(fused_norms) is not bool:
+        raise ValueError("fused_norms must be a bool")
     engine, _, counters, linear_cls = load_runtime()
     fp4 = precision == "fp4"
     if fp4:
@@ -63,7 +87,9 @@ def prepare(model, *, profile, precision, remat, lr, betas, eps, weight_decay):
         model = model.cuda()
     model, opt = engine.configure(model, precision, cfg.storage, lr=lr, tiles=cfg.tiles, warps=cfg.warps, direct=direct, remat=remat,
                                   act_pair=fp4, fast_scale=fp4, mma_k=128 if fp4 and cfg.short_mma_warps else 0,
-                                  mma_warps=cfg.short_mma_warps or 8)
+                                  mma_warps=cfg.short_mma_warps or 8, fp8_layers=fp8_layers)
+    if fused_norms:
+        _fuse_norms(model)
     if fp4:
         for module in model.modules():
             if isinstance(module, engine.Linear6):

@@ -40,7 +40,8 @@ class GradientReducer:
         self.depth = max(0, int(depth))
         self.slot_dtype = slot_dtype
         self._slots = {}
-        owners = [p for p in params if (owner_filter(p) if owner_filter else getattr(p, "_v4_request_scale", False))]
+        owners = [p for p in params if (owner_filter(p) if owner_filter else getattr(p, "_v4_request_scale", False) or
+                                        (getattr(p, "_v6_defer_dense", False) and p.numel() >= 4096))]
         for p in owners:
             self._slots[p] = torch.zeros(p.numel(), dtype=slot_dtype, device=p.device)
         self._works = []          # eager mode: outstanding collectives

@@ -154,3 +154,17 @@ def test_fp8_entry_points_refuse_before_any_launch():
     assert gemm(k=0) == 1 and gemm(m=1 << 30) == 1 and gemm(m=1 << 29, n=1 << 29, ldo=1 << 29) == 1
     assert gemm(od=3) == 3 and gemm(bias=at, bd=4) == 3 and gemm(a=at + 8) == 2 and gemm(out=at + 1) == 2
     assert lib.nvfp4_column_sums(at, 0, 8, at, 0, None) == 1 and lib.nvfp4_column_sums(at, 1, 8, at, 3, None) == 3
+
+
+def test_data_parallel_slots_hold_the_8_bit_weights(tmp_path):
+    import torch.distributed as dist
+    from nvfp4_training.distributed import GradientReducer
+    dist.init_process_group("gloo", init_method=f"file://{tmp_path}/store", rank=0, world_size=1)
+    try:
+        nvfp4, fp8, small, dense = (torch.nn.Parameter(torch.zeros(n)) for n in (5000, 4096, 64, 9000))
+        nvfp4._v4_request_scale = fp8._v6_defer_dense = small._v6_defer_dense = True
+        reducer = GradientReducer([nvfp4, fp8, small, dense])
+        assert [reducer.has_slot(p) for p in (nvfp4, fp8, small, dense)] == [True, True, False, False]
+        assert reducer.layout()[0] == (5000, 4096)
+    finally:
+        dist.destroy_process_group()
