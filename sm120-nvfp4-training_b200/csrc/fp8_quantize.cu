@@ -41,24 +41,36 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
     return static_cast<uint32_t>(lo) | static_cast<uint32_t>(hi) << 16;
 }
-__device__ __forceinline__ float warp_max_bits(float v, int from) {      // maximum of non-negative floats, NaN greatest
-    uint32_t b = __float_as_uint(v);
-    for (int d = from; d > 0; d >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, d));
-    return __uint_as_float(b);
-}
 __device__ __forceinline__ float max_bits(float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); }
 
 // E: elements per 16-byte vector; a row is L lanes, a warp holds 32 / L rows side by side and I of them per lane.
 template <typename T> struct Fp8Map {
     static constexpr int E = 16 / sizeof(T), L = 128 / E, I = 16 * L / 32;
+    static constexpr int CTAS = sizeof(T) == 2 ? 4 : 2;      // per SM: 32 or 64 registers hold the tile's share of a thread
 };
 
+// Magnitude maxima as integers: 16-bit types two to a register, FP32 one.
+template <typename T> struct Magnitude {
+    static constexpr int PER = sizeof(T) == 2 ? 2 : 1, WORDS = 4;      // per register; registers per 16-byte vector
+    static __device__ __forceinline__ uint32_t of(uint32_t w) { return w & (PER == 2 ? 0x7fff7fffu : 0x7fffffffu); }
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return PER == 2 ? __vmaxu2(a, b) : max(a, b); }
+    static __device__ __forceinline__ uint32_t single(uint32_t m) { return PER == 2 ? max(m & 0xffffu, m >> 16) : m; }      // of a register's two
+    static __device__ __forceinline__ float value(uint32_t bits) {     // FP32 of one element's magnitude bits
+        if constexpr (sizeof(T) == 4) return __uint_as_float(bits);
+        else if constexpr (Code<T>::value == NVFP4_BF16) return __uint_as_float(bits << 16);
+        else return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+    }
+};
+template <typename T, int E> __device__ __forceinline__ const uint32_t* words(const Pack<T, E>& v) { return reinterpret_cast<const uint32_t*>(&v); }
+
 template <typename T, bool COL, bool SQUARE>
-__global__ void __launch_bounds__(F8_THREADS) fp8_quantize_kernel(const Fp8Args a) {
+__global__ void __launch_bounds__(F8_THREADS, Fp8Map<T>::CTAS) fp8_quantize_kernel(const Fp8Args a) {
     using M = Fp8Map<T>;
+    using Mag = Magnitude<T>;
     constexpr int E = M::E, L = M::L, I = M::I;
     __shared__ __align__(16) uint8_t turned[COL ? 128 * 128 : 16];
-    __shared__ float warp_cols[COL ? 8 : 1][COL ? 128 : 1], col_inverse[128], warp_best[8];
+    __shared__ float warp_cols[COL ? 8 : 1][COL ? 128 : 1], col_inverse[128], row_inverse[128];
+    __shared__ uint32_t warp_best[8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
     const int64_t rb = blockIdx.x / a.col_blocks, cb = blockIdx.x - rb * a.col_blocks;
     const int cl = lane % L, part = lane / L;                 // column group, and which run of I rows of the warp's sixteen
@@ -80,42 +92,57 @@ __global__ void __launch_bounds__(F8_THREADS) fp8_quantize_kernel(const Fp8Args 
             }
         }
     }
-    float row_best[I], col_best[E];
-#pragma unroll
-    for (int j = 0; j < E; ++j) col_best[j] = 0.f;
+    uint32_t row_best[I];
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-        float f[E];
-        unpack(v[i], f);
-        row_best[i] = 0.f;
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-            row_best[i] = max_bits(row_best[i], fabsf(f[j]));
-            if (COL && !SQUARE) col_best[j] = max_bits(col_best[j], fabsf(f[j]));
-        }
+        const uint32_t* w = words(v[i]);
+        row_best[i] = Mag::larger(Mag::larger(Mag::of(w[0]), Mag::of(w[1])), Mag::larger(Mag::of(w[2]), Mag::of(w[3])));
     }
     Fp8Scale square{};
     if constexpr (SQUARE) {
-        float best = 0.f;
+        uint32_t best = row_best[0];
 #pragma unroll
-        for (int i = 0; i < I; ++i) best = max_bits(best, row_best[i]);
-        best = warp_max_bits(best, 16);
+        for (int i = 1; i < I; ++i) best = Mag::larger(best, row_best[i]);
+        best = __reduce_max_sync(0xffffffffu, Mag::single(best));
         if (lane == 0) warp_best[warp] = best;
         __syncthreads();
-        best = 0.f;
+        best = 0;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) best = max_bits(best, warp_best[w]);
-        square = fp8_scale(best);
+        for (int w = 0; w < 8; ++w) best = max(best, warp_best[w]);
+        square = fp8_scale(Mag::value(best));
+    } else if (a.codes) {
+        // The I rows' maxima over their L lanes, halving the rows a lane carries at each exchange: afterwards lane cl holds
+        // the maximum of row cl * I / L of its run, forms its scale once, and the run's lanes read it from shared memory.
+#pragma unroll
+        for (int d = L / 2, n = I; d > 0; d >>= 1) {
+            if (n > 1) {
+                n >>= 1;
+                const bool upper = cl & d;
+#pragma unroll
+                for (int i = 0; i < n; ++i) {
+                    const uint32_t keep = upper ? row_best[i + n] : row_best[i], send = upper ? row_best[i] : row_best[i + n];
+                    row_best[i] = Mag::larger(keep, __shfl_xor_sync(0xffffffffu, send, d));
+                }
+            } else {
+                row_best[0] = Mag::larger(row_best[0], __shfl_xor_sync(0xffffffffu, row_best[0], d));
+            }
+        }
+        const Fp8Scale s = fp8_scale(Mag::value(Mag::single(row_best[0])));
+        if (cl % (L / I) == 0) {
+            const int r = row_in + cl / (L / I);
+            row_inverse[r] = s.inverse;
+            *reinterpret_cast<uint32_t*>(a.scales + (rb * a.col_blocks + cb) * 512 + (r & 31) * 16 + (r >> 5) * 4) = s.word;
+        }
+        __syncwarp();
     }
     if (COL && a.column_sums) {                                // each lane's rows, then the warps' in order
-        float sum[E];
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-            sum[j] = 0.f;
+            float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < I; ++i) sum[j] += to_float(v[i].e[j]);
-            if (L == 16) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 16);
-            if (part == 0) warp_cols[warp][col_in + j] = sum[j];
+            for (int i = 0; i < I; ++i) sum += to_float(v[i].e[j]);
+            if (L == 16) sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+            if (part == 0) warp_cols[warp][col_in + j] = sum;
         }
         __syncthreads();
         if (tid < 128 && cb * 128 + tid < a.cols) {
@@ -128,24 +155,29 @@ __global__ void __launch_bounds__(F8_THREADS) fp8_quantize_kernel(const Fp8Args 
     }
     if constexpr (COL && !SQUARE) {
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-            if (L == 16) col_best[j] = max_bits(col_best[j], __shfl_xor_sync(0xffffffffu, col_best[j], 16));
-            if (part == 0) warp_cols[warp][col_in + j] = col_best[j];
+        for (int k = 0; k < 4; ++k) {
+            uint32_t best = Mag::of(words(v[0])[k]);
+#pragma unroll
+            for (int i = 1; i < I; ++i) best = Mag::larger(best, Mag::of(words(v[i])[k]));
+            if (L == 16) best = Mag::larger(best, __shfl_xor_sync(0xffffffffu, best, 16));
+            if (part == 0) {
+                if constexpr (Mag::PER == 2) {
+                    warp_cols[warp][col_in + 2 * k] = Mag::value(best & 0xffffu);
+                    warp_cols[warp][col_in + 2 * k + 1] = Mag::value(best >> 16);
+                } else {
+                    warp_cols[warp][col_in + k] = Mag::value(best);
+                }
+            }
         }
     }
     if (a.codes) {
 #pragma unroll
         for (int i = 0; i < I; ++i) {
-            Fp8Scale s = square;
-            if (!SQUARE) s = fp8_scale(warp_max_bits(row_best[i], L / 2));
-            if (!SQUARE && cl == (i & (L - 1))) {
-                const int r = row_in + i;
-                *reinterpret_cast<uint32_t*>(a.scales + (rb * a.col_blocks + cb) * 512 + (r & 31) * 16 + (r >> 5) * 4) = s.word;
-            }
+            const float inverse = SQUARE ? square.inverse : row_inverse[row_in + i];
             float f[E];
             unpack(v[i], f);
 #pragma unroll
-            for (int j = 0; j < E; ++j) f[j] *= s.inverse;
+            for (int j = 0; j < E; ++j) f[j] *= inverse;
             if (row0 + i < a.rows) {
                 uint8_t* out = a.codes + (row0 + i) * a.cols_p + col0;
                 if constexpr (E == 8) *reinterpret_cast<uint2*>(out) = make_uint2(e4m3x4(f[0], f[1], f[2], f[3]), e4m3x4(f[4], f[5], f[6], f[7]));
