@@ -345,12 +345,13 @@ int nvfp4_comfy_rope(const void* x, const void* rotation, void* out, int64_t row
  */
 int nvfp4_layer_norm(const void* x, int x_dtype, int64_t x_pitch, const void* delta, int delta_dtype, int64_t delta_pitch,
                      const void* weight, const void* bias, int weight_dtype, float eps, int64_t rows, int64_t cols, void* sum_out,
-                     void* h_out, int h_dtype, float* mean_out, float* rstd_out, float* amax, nvfp4_stream_t stream);
+                     void* h_out, int h_dtype, float* mean_out, float* rstd_out, float* amax, int* status,
+                     nvfp4_stream_t stream);
 int64_t nvfp4_layer_norm_bwd_partials(int64_t rows, int64_t cols);
 int nvfp4_layer_norm_bwd(const void* dh, int h_dtype, int64_t dh_pitch, const void* total, int x_dtype, int64_t total_pitch,
                          const float* mean, const float* rstd, const void* weight, int weight_dtype, const void* dsum,
                          int64_t dsum_pitch, int64_t rows, int64_t cols, void* dx, void* ddelta, float* partial, void* dweight,
-                         void* dbias, float* amax, nvfp4_stream_t stream);
+                         void* dbias, float* amax, int* status, nvfp4_stream_t stream);
 
 /*
  * nvfp4_rotary_axes: up to three tensors [batch][seq][heads][dim] (strides of batch, seq and head in elements, features

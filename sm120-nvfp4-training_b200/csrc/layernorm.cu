@@ -8,6 +8,7 @@
 // one CTA above that; the centred second sweep keeps the variance exact where the mean is large against the spread.  All
 // statistics are FP32; a result is rounded once, except that h is formed from the total as it is stored (the backward pass
 // reads that one too).
+#include "async.cuh"
 #include "bf16x8.cuh"
 #include "vec.cuh"
 
@@ -19,6 +20,7 @@ struct NormArgs {
     const void *x, *delta, *weight, *bias;
     void *sum, *h;
     float *mean, *rstd, *amax;
+    int* status;
     int64_t x_pitch, delta_pitch, rows;
     int cols, delta_bf16, weight_dtype;   // delta_bf16: a BF16 delta beside an FP32 x
     float eps;
@@ -37,12 +39,12 @@ __device__ __forceinline__ float cta_sum(float v, float* slots) {
 // V elements of total at column c of row r (stored, too, when there is a delta), as FP32
 template <typename TX, int V>
 __device__ __forceinline__ void load_total(const NormArgs& a, int64_t r, int c, float (&f)[V]) {
-    Pack<TX, V> p = load_pack<TX, V>(static_cast<const TX*>(a.x) + r * a.x_pitch + c);
+    Pack<TX, V> p = load_const<TX, V>(static_cast<const TX*>(a.x) + r * a.x_pitch + c);
     unpack(p, f);
     if (a.delta) {
         float d[V];
-        if (sizeof(TX) == 4 && a.delta_bf16) unpack(load_pack<__nv_bfloat16, V>(static_cast<const __nv_bfloat16*>(a.delta) + r * a.delta_pitch + c), d);
-        else unpack(load_pack<TX, V>(static_cast<const TX*>(a.delta) + r * a.delta_pitch + c), d);
+        if (sizeof(TX) == 4 && a.delta_bf16) unpack(load_const<__nv_bfloat16, V>(static_cast<const __nv_bfloat16*>(a.delta) + r * a.delta_pitch + c), d);
+        else unpack(load_const<TX, V>(static_cast<const TX*>(a.delta) + r * a.delta_pitch + c), d);
 #pragma unroll
         for (int j = 0; j < V; ++j) f[j] += d[j];
         p = pack<TX, V>(f);
@@ -67,7 +69,7 @@ __device__ __forceinline__ float store_normed(const NormArgs& a, int64_t r, int 
     }
     const Pack<TO, V> q = pack<TO, V>(o);
     store_pack(static_cast<TO*>(a.h) + r * a.cols + c, q);
-    return abs_max(q);
+    return a.amax ? abs_max(q) : 0.f;
 }
 
 // N vectors of V elements per thread; ROW_CTA: a CTA per row, else a warp per row.
@@ -145,6 +147,7 @@ struct NormBwdArgs {
     const void *dh, *total, *weight, *dsum;
     const float *mean, *rstd;
     void *dx, *ddelta;
+    int* status;
     float *partial, *amax;     // partial: [parts][2][cols], null when neither dw nor db is asked for
     int64_t dh_pitch, total_pitch, dsum_pitch, rows;
     int cols, weight_dtype;
@@ -155,8 +158,9 @@ template <typename TX, int V>
 __device__ __forceinline__ float store_dx(const NormBwdArgs& a, int64_t r, int c, const float (&u)[V], const float (&z)[V], float rstd,
                                           float mean_u, float mean_uz, const Pack<TX, V>& dsum) {
     float o[V], d[V];
+    const float k1 = -rstd * mean_u, k2 = -rstd * mean_uz;
 #pragma unroll
-    for (int j = 0; j < V; ++j) o[j] = rstd * (u[j] - mean_u - z[j] * mean_uz);
+    for (int j = 0; j < V; ++j) o[j] = fmaf(u[j], rstd, fmaf(z[j], k2, k1));
     if (a.dsum) {
         unpack(dsum, d);
 #pragma unroll
@@ -167,9 +171,9 @@ __device__ __forceinline__ float store_dx(const NormBwdArgs& a, int64_t r, int c
     if (sizeof(TX) == 4 && a.ddelta) {
         const Pack<__nv_bfloat16, V> qd = pack<__nv_bfloat16, V>(o);
         store_pack(static_cast<__nv_bfloat16*>(a.ddelta) + r * a.cols + c, qd);
-        return abs_max(qd);
+        return a.amax ? abs_max(qd) : 0.f;
     }
-    return abs_max(q);
+    return a.amax ? abs_max(q) : 0.f;
 }
 
 // Every thread owns N vectors of V columns for all rows its group (a warp, or the CTA) takes, so the column sums stay in
@@ -364,31 +368,424 @@ __global__ void __launch_bounds__(256) norm_bwd_columns_kernel(const NormBwdArgs
 }
 
 // out[c] = sum of `parts` rows of `width` floats, columns [0, cols) to out0 and [cols, 2 cols) to out1 (either may be null).
-// A CTA takes 32 columns, its eight warps every eighth row each, the eight subtotals are added in warp order.
-__global__ void __launch_bounds__(256) column_sums_kernel(const float* __restrict__ partial, int64_t parts, int64_t width, int64_t cols,
-                                                          void* out0, void* out1, int dtype) {
-    __shared__ float subtotal[8][32];
+// A CTA takes 32 columns, its 32 warps every 32nd row each, the subtotals are added in warp order.
+__global__ void __launch_bounds__(1024) column_sums_kernel(const float* __restrict__ partial, int64_t parts, int64_t width, int64_t cols,
+                                                           void* out0, void* out1, int dtype) {
+    __shared__ float subtotal[32][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
     float t = 0.f;
     if (c < width) {
 #pragma unroll 8
-        for (int64_t p = warp; p < parts; p += 8) t += partial[p * width + c];
+        for (int64_t p = warp; p < parts; p += 32) t += partial[p * width + c];
     }
     subtotal[warp][lane] = t;
     __syncthreads();
-    if (warp != 0 || c >= width) return;
-    float total = 0.f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) total += subtotal[w][lane];
-    void* out = c < cols ? out0 : out1;
-    if (out) store_param(out, dtype, c < cols ? c : c - cols, total);
+    const int64_t mine = static_cast<int64_t>(blockIdx.x) * 32 + warp;        // a warp adds one column's subtotals
+    t = warp_sum(subtotal[lane][warp]);
+    void* out = mine < cols ? out0 : out1;
+    if (lane == 0 && mine < width && out) store_param(out, dtype, mine < cols ? mine : mine - cols, t);
 }
 
-constexpr int64_t NORM_MAX_PARTS = 148 * 4;
+// ====================================================================================================================
+// rows through a ring in shared memory
+// ====================================================================================================================
+// With its operands in registers alone a CTA loads a row, waits, reduces, waits, and stores: 0.3 to 0.6 of HBM, all of it load
+// latency (long-scoreboard stalls 10 of 16 cycles per instruction).  Here one thread keeps bulk copies of the next rows in
+// flight into a ring of stages, and a stage is refilled as soon as the CTA's first barrier behind its reads has passed.  CTAs
+// are persistent, so weight and bias (and the backward pass's column sums) stay in registers: eight columns per thread, as
+// one 16-byte vector of a 16-bit x or two of an FP32 one, up to 8192 columns.  Narrow rows have several groups of threads side
+// by side in a CTA; R rows of each group share the barriers of a round.
+namespace ring {
+constexpr int MAX_STAGES = 8;
+constexpr int BYTES_PER_SM = 216 * 1024;
+struct Plan { int row_threads, threads, stages, stage_bytes, ctas; };
+}  // namespace ring
+
+struct RingOperand { const uint8_t* base; int64_t pitch; uint32_t bytes; };       // pitch and row length in bytes; base null: absent
+
+// Runs of `per_stage` rows of up to OPS operands through the ring; thread 0 is the producer.  What only it needs lies in shared
+// memory (held in registers by every thread it cost 20 of them).  Every wait is bounded: when one runs out, all later ones
+// return at once, the loops end over stale data, and the status word says so.
+template <int OPS>
+struct RowRing {
+    RingOperand op[OPS];
+    int64_t rows, groups;
+    uint32_t row_bytes;
+    int per_stage, stages, abort_flag;
+    uint64_t full[ring::MAX_STAGES];
+};
+struct RingCursor { int slot; uint32_t phase; };
+
+template <int OPS>
+__device__ __forceinline__ void ring_fill(RowRing<OPS>& q, uint8_t* data, int64_t group, int into) {
+    const int64_t r0 = group * q.per_stage;
+    const int live = static_cast<int>(q.rows - r0 < q.per_stage ? q.rows - r0 : q.per_stage);
+    aop::mbar_expect_tx(&q.full[into], live * q.row_bytes);
+    uint8_t* dst = data + static_cast<size_t>(into) * q.per_stage * q.row_bytes;
+    for (int o = 0; o < OPS; ++o) {
+        const RingOperand op = q.op[o];
+        if (!op.base) continue;
+        const uint8_t* src = op.base + r0 * op.pitch;
+        if (op.pitch == op.bytes) aop::bulk_load(dst, src, live * op.bytes, &q.full[into]);
+        else for (int k = 0; k < live; ++k) aop::bulk_load(dst + k * op.bytes, src + k * op.pitch, op.bytes, &q.full[into]);
+        dst += q.per_stage * op.bytes;
+    }
+}
+// by thread 0, which has set the operands, rows, per_stage and stages
+template <int OPS>
+__device__ __forceinline__ void ring_start(RowRing<OPS>& q, uint8_t* data) {
+    q.groups = (q.rows + q.per_stage - 1) / q.per_stage;
+    q.row_bytes = 0;
+    for (int o = 0; o < OPS; ++o) q.row_bytes += q.op[o].base ? q.op[o].bytes : 0;
+    for (int s = 0; s < q.stages; ++s) aop::mbar_init(&q.full[s], 1);
+    q.abort_flag = 0;
+    aop::fence_barrier_init();
+    for (int s = 0; s < q.stages; ++s) {
+        const int64_t group = blockIdx.x + static_cast<int64_t>(s) * gridDim.x;
+        if (group < q.groups) ring_fill(q, data, group, s);
+    }
+}
+// behind a barrier that follows every read of the present stage
+template <int OPS>
+__device__ __forceinline__ void ring_advance(RowRing<OPS>& q, uint8_t* data, RingCursor& at, int stages, int64_t group) {
+    if (threadIdx.x == 0) {
+        const int64_t next = group + static_cast<int64_t>(stages) * gridDim.x;
+        if (next < q.groups && !*static_cast<volatile int*>(&q.abort_flag)) ring_fill(q, data, next, at.slot);
+    }
+    if (++at.slot == stages) { at.slot = 0; at.phase ^= 1; }
+}
+// after the last barrier: a bounded wait for copies that nobody read
+template <int OPS>
+__device__ __forceinline__ void ring_finish(RowRing<OPS>& q, int* status) {
+    if (threadIdx.x == 0 && *static_cast<volatile int*>(&q.abort_flag)) {
+        const long long t0 = clock64();
+        for (int s = 0; s < q.stages; ++s)
+            while (!aop::mbar_try(&q.full[s], 0) && !aop::mbar_try(&q.full[s], 1) && clock64() - t0 < aop::WAIT_LIMIT_CYCLES / 8) {}
+        while (clock64() - t0 < 400000) {}
+        if (status) atomicExch(status, NVFP4_ERR_TIMEOUT);
+    }
+}
+
+// C sums over a group of `warps` warps from `first` on, in a fixed order; every thread gets all of them; one barrier of the CTA
+// (see cta_sum).  The lanes of a warp fold the C values together, halving what each carries at every exchange, so that lane l
+// ends with the warp's sum of value l C / 32; each warp then adds the group's warps, 32 / C at a time.
+template <int C>
+__device__ __forceinline__ void group_sums(float (&a)[C], float (*slots)[C], int first, int warps) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int d = 16, n = C; d > 0; d >>= 1) {
+        if (n > 1) {
+            n >>= 1;
+            const bool upper = lane & d;
+#pragma unroll
+            for (int i = 0; i < n; ++i) {
+                const float keep = upper ? a[i + n] : a[i], send = upper ? a[i] : a[i + n];
+                a[i] = keep + __shfl_xor_sync(0xffffffffu, send, d);
+            }
+        } else {
+            a[0] += __shfl_xor_sync(0xffffffffu, a[0], d);
+        }
+    }
+    if (lane % (32 / C) == 0) slots[threadIdx.x >> 5][lane / (32 / C)] = a[0];
+    __syncthreads();
+    float t = 0.f;
+    for (int w = lane / C; w < warps; w += 32 / C) t += slots[first + w][lane % C];
+#pragma unroll
+    for (int d = C; d < 32; d <<= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
+#pragma unroll
+    for (int i = 0; i < C; ++i) a[i] = __shfl_sync(0xffffffffu, t, i);
+}
+
+template <typename T, int V> __device__ __forceinline__ void load_or(const void* p, int dtype, int c, bool live, float otherwise, T (&f)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = otherwise;
+    if (p && live) load_param<V>(p, dtype, c, f);
+}
+
+template <typename TX, typename TD, typename TO, int R, int MAXT>
+__global__ void __launch_bounds__(MAXT, MAXT == 256 ? 4 : MAXT == 640 ? 2 : 1) norm_fwd_ring_kernel(const NormArgs a, int stages, int row_threads) {
+    constexpr int V = 16 / sizeof(TX), N = 8 / V;
+    extern __shared__ __align__(128) uint8_t ring_data[];
+    __shared__ float slots[2][32][R];
+    __shared__ RowRing<2> q;
+    const int group = threadIdx.x / row_threads, tid = threadIdx.x - group * row_threads, step = row_threads, vectors = a.cols / V;
+    const int per_stage = blockDim.x / row_threads * R, first_warp = group * (row_threads >> 5);
+    const uint32_t x_bytes = a.cols * sizeof(TX), d_bytes = a.delta ? a.cols * sizeof(TD) : 0;
+    if (threadIdx.x == 0) {
+        q.op[0] = {static_cast<const uint8_t*>(a.x), a.x_pitch * static_cast<int64_t>(sizeof(TX)), x_bytes};
+        q.op[1] = {static_cast<const uint8_t*>(a.delta), a.delta_pitch * static_cast<int64_t>(sizeof(TD)), d_bytes};
+        q.rows = a.rows;
+        q.per_stage = per_stage;
+        q.stages = stages;
+        ring_start(q, ring_data);
+    }
+    __syncthreads();
+    const int64_t runs = q.groups;
+    const uint32_t stage_bytes = per_stage * q.row_bytes;
+    RingCursor at{0, 0};
+    float w[N][V], b[N][V];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int c = tid + i * step;
+        load_or(a.weight, a.weight_dtype, c * V, c < vectors, 1.f, w[i]);
+        load_or(a.bias, a.weight_dtype, c * V, c < vectors, 0.f, b[i]);
+    }
+    const float inv_n = 1.f / static_cast<float>(a.cols);
+    float best = 0.f;
+    for (int64_t g = blockIdx.x; g < runs; g += gridDim.x) {
+        aop::mbar_wait(&q.full[at.slot], at.phase, &q.abort_flag);
+        const uint8_t* stage = ring_data + at.slot * stage_bytes;
+        float f[R][N][V], sums[R];
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            const int64_t r = g * per_stage + group * R + k;
+            sums[k] = 0.f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = tid + i * step;
+                if (c >= vectors || r >= a.rows) continue;
+                unpack(load_pack<TX, V>(reinterpret_cast<const TX*>(stage + (group * R + k) * x_bytes) + c * V), f[k][i]);
+                if (a.delta) {
+                    float d[V];
+                    unpack(load_pack<TD, V>(reinterpret_cast<const TD*>(stage + per_stage * x_bytes + (group * R + k) * d_bytes) + c * V), d);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) f[k][i][j] += d[j];
+                    const Pack<TX, V> p = pack<TX, V>(f[k][i]);
+                    store_pack(static_cast<TX*>(a.sum) + r * a.cols + c * V, p);
+                    unpack(p, f[k][i]);
+                }
+#pragma unroll
+                for (int j = 0; j < V; ++j) sums[k] += f[k][i][j];
+            }
+        }
+        group_sums(sums, slots[0], first_warp, step >> 5);
+        ring_advance(q, ring_data, at, stages, g);
+        float mean[R];
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            mean[k] = sums[k] * inv_n;
+            sums[k] = 0.f;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (tid + i * step < vectors) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) { const float d = f[k][i][j] - mean[k]; sums[k] = fmaf(d, d, sums[k]); }
+                }
+        }
+        group_sums(sums, slots[1], first_warp, step >> 5);
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            const int64_t r = g * per_stage + group * R + k;
+            if (r >= a.rows) continue;
+            const float rstd = rsqrtf(sums[k] * inv_n + a.eps);
+            if (tid == 0 && a.mean) { a.mean[r] = mean[k]; a.rstd[r] = rstd; }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = tid + i * step;
+                if (c >= vectors) continue;
+                float o[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) o[j] = fmaf((f[k][i][j] - mean[k]) * rstd, w[i][j], b[i][j]);
+                const Pack<TO, V> q = pack<TO, V>(o);
+                store_pack(static_cast<TO*>(a.h) + r * a.cols + c * V, q);
+                if (a.amax) best = fmaxf(best, abs_max(q));
+            }
+        }
+    }
+    if (a.amax) block_atomic_amax(a.amax, best);
+    ring_finish(q, a.status);
+}
+
+template <typename TX, typename TH, int R, int MAXT>
+__global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) norm_bwd_ring_kernel(const NormBwdArgs a, int stages, int row_threads) {
+    constexpr int V = 16 / sizeof(TX), N = 8 / V;
+    extern __shared__ __align__(128) uint8_t ring_data[];
+    __shared__ float slots[2][32][2 * R];
+    __shared__ RowRing<3> q;
+    const int group = threadIdx.x / row_threads, tid = threadIdx.x - group * row_threads, step = row_threads, vectors = a.cols / V;
+    const int per_stage = blockDim.x / row_threads * R, first_warp = group * (row_threads >> 5);
+    const uint32_t h_bytes = a.cols * sizeof(TH), x_bytes = a.cols * sizeof(TX), s_bytes = a.dsum ? x_bytes : 0;
+    if (threadIdx.x == 0) {
+        q.op[0] = {static_cast<const uint8_t*>(a.dh), a.dh_pitch * static_cast<int64_t>(sizeof(TH)), h_bytes};
+        q.op[1] = {static_cast<const uint8_t*>(a.total), a.total_pitch * static_cast<int64_t>(sizeof(TX)), x_bytes};
+        q.op[2] = {static_cast<const uint8_t*>(a.dsum), a.dsum_pitch * static_cast<int64_t>(sizeof(TX)), s_bytes};
+        q.rows = a.rows;
+        q.per_stage = per_stage;
+        q.stages = stages;
+        ring_start(q, ring_data);
+    }
+    __syncthreads();
+    const int64_t runs = q.groups;
+    const uint32_t stage_bytes = per_stage * q.row_bytes;
+    RingCursor at{0, 0};
+    float w[N][V], acc_w[N][V], acc_b[N][V];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        load_or(a.weight, a.weight_dtype, (tid + i * step) * V, tid + i * step < vectors, 1.f, w[i]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc_w[i][j] = acc_b[i][j] = 0.f;
+    }
+    const float inv_n = 1.f / static_cast<float>(a.cols);
+    float best = 0.f, mean[R], rstd[R];          // of the next group, fetched one round ahead
+    auto statistics = [&](int64_t g) {
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            const int64_t r = g * per_stage + group * R + k;
+            mean[k] = r < a.rows ? __ldg(a.mean + r) : 0.f;
+            rstd[k] = r < a.rows ? __ldg(a.rstd + r) : 0.f;
+        }
+    };
+    statistics(blockIdx.x);
+    int half = 0;
+    for (int64_t g = blockIdx.x; g < runs; g += gridDim.x, half ^= 1) {
+        aop::mbar_wait(&q.full[at.slot], at.phase, &q.abort_flag);
+        const uint8_t* stage = ring_data + at.slot * stage_bytes;
+        float u[R][N][V], z[R][N][V], sums[2 * R], rs[R];
+        Pack<TX, V> res[R][N];
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            rs[k] = rstd[k];
+            const float shift = -mean[k] * rstd[k];
+            sums[2 * k] = sums[2 * k + 1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = tid + i * step, row = group * R + k;
+                if (c >= vectors || g * per_stage + row >= a.rows) continue;
+                unpack(load_pack<TH, V>(reinterpret_cast<const TH*>(stage + row * h_bytes) + c * V), u[k][i]);
+                unpack(load_pack<TX, V>(reinterpret_cast<const TX*>(stage + per_stage * h_bytes + row * x_bytes) + c * V), z[k][i]);
+                if (a.dsum) res[k][i] = load_pack<TX, V>(reinterpret_cast<const TX*>(stage + per_stage * (h_bytes + x_bytes) + row * s_bytes) + c * V);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float dh = u[k][i][j];
+                    z[k][i][j] = fmaf(z[k][i][j], rs[k], shift);
+                    acc_w[i][j] = fmaf(dh, z[k][i][j], acc_w[i][j]);
+                    acc_b[i][j] += dh;
+                    u[k][i][j] = dh * w[i][j];
+                    sums[2 * k] += u[k][i][j];
+                    sums[2 * k + 1] = fmaf(u[k][i][j], z[k][i][j], sums[2 * k + 1]);
+                }
+            }
+        }
+        statistics(g + gridDim.x);
+        group_sums(sums, slots[half], first_warp, step >> 5);
+        ring_advance(q, ring_data, at, stages, g);
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            const int64_t r = g * per_stage + group * R + k;
+            if (r >= a.rows) continue;
+            const float mean_u = sums[2 * k] * inv_n, mean_uz = sums[2 * k + 1] * inv_n;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = tid + i * step;
+                if (c < vectors) best = fmaxf(best, store_dx<TX, V>(a, r, c * V, u[k][i], z[k][i], rs[k], mean_u, mean_uz, res[k][i]));
+            }
+        }
+    }
+    if (a.amax) block_atomic_amax(a.amax, best);
+    ring_finish(q, a.status);
+    if (!a.partial) return;
+    // the groups' sums meet in shared memory (the ring is empty) and are added in group order
+    float* out = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
+    const bool alone = step == blockDim.x;
+    float* meet = reinterpret_cast<float*>(ring_data) + static_cast<int64_t>(group) * 2 * a.cols;
+    float* mine = alone ? out : meet;
+    if (!alone) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int c = tid + i * step;
+        if (c >= vectors) continue;
+        store_pack(mine + c * V, pack<float, V>(acc_w[i]));
+        store_pack(mine + a.cols + c * V, pack<float, V>(acc_b[i]));
+    }
+    if (alone) return;
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * a.cols; c += blockDim.x) {
+        float t = 0.f;
+        for (int q = 0; q < static_cast<int>(blockDim.x) / step; ++q) t += reinterpret_cast<const float*>(ring_data)[static_cast<int64_t>(q) * 2 * a.cols + c];
+        out[c] = t;
+    }
+}
+
+constexpr int64_t NORM_MAX_PARTS = 148 * 6;
 constexpr int64_t MAX_GRID = 1 << 30;
 
 static int round32(int n) { return (n + 31) / 32 * 32; }
+
+// Threads for eight columns each, narrow rows in groups that make 256 threads; as many CTAs per SM as give about 1024 threads
+// and leave each of them three stages.
+static int row_threads_for(int64_t cols) { return round32(static_cast<int>((cols + 7) / 8)); }
+static ring::Plan ring_plan(int64_t rows, int64_t cols, int rows_per_group, int row_bytes, int sms, int threads_per_sm, bool backward) {
+    ring::Plan p;
+    p.row_threads = row_threads_for(cols);
+    // few rows: no group without one
+    const int64_t want = std::max<int64_t>(1, (rows + static_cast<int64_t>(rows_per_group) * sms - 1) / (static_cast<int64_t>(rows_per_group) * sms));
+    const int groups = static_cast<int>(std::min<int64_t>(std::max(1, 256 / p.row_threads), want));
+    p.threads = p.row_threads * groups;
+    p.stage_bytes = groups * rows_per_group * row_bytes;
+    p.ctas = std::max(1, std::min(threads_per_sm / p.threads, ring::BYTES_PER_SM / (3 * p.stage_bytes + 2048)));
+    p.stages = std::max(2, std::min(ring::MAX_STAGES, (ring::BYTES_PER_SM / p.ctas - 2048) / p.stage_bytes));
+    // the groups' column sums of the backward pass (8 bytes a column) fit the stages: a row alone is 4 bytes a column or more
+    if (backward) while (p.stages * p.stage_bytes < groups * 8 * cols) ++p.stages;
+    const int64_t all = (rows + static_cast<int64_t>(groups) * rows_per_group - 1) / (static_cast<int64_t>(groups) * rows_per_group);
+    p.ctas = static_cast<int>(std::min<int64_t>({all, static_cast<int64_t>(p.ctas) * sms, NORM_MAX_PARTS}));
+    return p;
+}
+static bool ring_operand(const void* p, int dtype, int64_t pitch, int64_t cols) {       // rows that bulk copies can fetch
+    return !p || (aligned(p, 16) && pitch * dtype_size(dtype) % 16 == 0 && cols * dtype_size(dtype) % 16 == 0);
+}
+static int sm_count() {
+    static int count[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return 148;
+    if (!count[dev]) cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev);
+    return count[dev];
+}
+// One launch of a ring kernel; KERNEL's shared-memory limit is raised once per device.
+template <typename Args>
+static bool launch_ring(void (*kernel)(Args, int, int), bool (&ready)[64], const Args& a, const ring::Plan& p, cudaStream_t st) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return false;
+    if (!ready[dev]) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring::BYTES_PER_SM) != cudaSuccess) return false;
+        ready[dev] = true;
+    }
+    kernel<<<p.ctas, p.threads, p.stages * p.stage_bytes, st>>>(a, p.stages, p.row_threads);
+    return true;
+}
+template <typename TX, typename TD, typename TO, int R, int MAXT>
+static bool fwd_ring(const NormArgs& a, const ring::Plan& p, cudaStream_t st) {
+    static bool ready[64] = {};
+    return launch_ring<NormArgs>(norm_fwd_ring_kernel<TX, TD, TO, R, MAXT>, ready, a, p, st);
+}
+template <typename TX, typename TD, typename TO>
+static bool fwd_ring_sized(const NormArgs& a, cudaStream_t st) {
+    const int row_bytes = a.cols * static_cast<int>(sizeof(TX) + (a.delta ? sizeof(TD) : 0));
+    // two rows a round where the rows are short; above 256 threads one, in two CTAs of up to 48 registers a thread
+    const int threads = row_threads_for(a.cols), r = threads <= 256 ? 2 : 1;
+    const ring::Plan p = ring_plan(a.rows, a.cols, r, row_bytes, sm_count(), r == 2 ? 1024 : 1344, false);
+    if (threads <= 256) return fwd_ring<TX, TD, TO, 2, 256>(a, p, st);
+    if (threads <= 640) return fwd_ring<TX, TD, TO, 1, 640>(a, p, st);
+    return fwd_ring<TX, TD, TO, 1, 1024>(a, p, st);
+}
+template <typename TX, typename TH, int R, int MAXT>
+static int64_t bwd_ring(const NormBwdArgs& a, const ring::Plan& p, cudaStream_t st) {
+    static bool ready[64] = {};
+    return launch_ring<NormBwdArgs>(norm_bwd_ring_kernel<TX, TH, R, MAXT>, ready, a, p, st) ? p.ctas : 0;
+}
+template <typename TX, typename TH>
+static int64_t bwd_ring_sized(const NormBwdArgs& a, cudaStream_t st) {
+    const int row_bytes = a.cols * static_cast<int>(sizeof(TH) + sizeof(TX) * (a.dsum ? 2 : 1));
+    // two rows a round where two stages of two rows fit
+    const int threads = row_threads_for(a.cols), r = threads <= 768 && 4 * row_bytes <= ring::BYTES_PER_SM - 2048 ? 2 : 1;
+    const ring::Plan p = ring_plan(a.rows, a.cols, r, row_bytes, sm_count(), 1024, true);
+    if (r == 1) return bwd_ring<TX, TH, 1, 1024>(a, p, st);
+    if (threads <= 256) return bwd_ring<TX, TH, 2, 256>(a, p, st);
+    if (threads <= 512) return bwd_ring<TX, TH, 2, 512>(a, p, st);
+    return bwd_ring<TX, TH, 2, 768>(a, p, st);
+}
 
 template <typename TX, typename TO, int V>
 static bool launch_fwd(const NormArgs& a, cudaStream_t st) {
@@ -407,8 +804,15 @@ static bool launch_fwd(const NormArgs& a, cudaStream_t st) {
 }
 
 template <typename TX, typename TO>
-static void forward(const NormArgs& a, bool vector, cudaStream_t st) {
+static void forward(const NormArgs& a, bool vector, bool ring, cudaStream_t st) {
     constexpr int V = 16 / sizeof(TX);
+    if (ring) {
+        if constexpr (sizeof(TX) == 4) {
+            if (a.delta_bf16 ? fwd_ring_sized<TX, __nv_bfloat16, TO>(a, st) : fwd_ring_sized<TX, TX, TO>(a, st)) return;
+        } else if (fwd_ring_sized<TX, TX, TO>(a, st)) {
+            return;
+        }
+    }
     if (vector ? launch_fwd<TX, TO, V>(a, st) : launch_fwd<TX, TO, 1>(a, st)) return;
     norm_fwd_any_kernel<TX, TO><<<static_cast<unsigned>(std::min(a.rows, MAX_GRID)), 256, 0, st>>>(a);
 }
@@ -438,13 +842,15 @@ static int64_t launch_bwd(const NormBwdArgs& a, cudaStream_t st) {
 }
 
 template <typename TX, typename TH>
-static int64_t backward(const NormBwdArgs& a, bool vector, cudaStream_t st) {
+static int64_t backward(const NormBwdArgs& a, bool vector, bool ring, cudaStream_t st) {
     constexpr int V = 16 / sizeof(TX);
+    if (ring)
+        if (const int64_t parts = bwd_ring_sized<TX, TH>(a, st)) return parts;
     if (const int64_t parts = vector ? launch_bwd<TX, TH, V>(a, st) : launch_bwd<TX, TH, 1>(a, st)) return parts;
     norm_bwd_any_kernel<TX, TH><<<static_cast<unsigned>(std::min(a.rows, MAX_GRID)), 256, 0, st>>>(a);
     if (!a.partial) return 1;
     const int64_t blocks = (a.cols + 31) / 32;
-    const int64_t parts = std::min<int64_t>({(a.rows + 31) / 32, NORM_MAX_PARTS, std::max<int64_t>(1, 148 * 16 / blocks)});
+    const int64_t parts = std::min<int64_t>({(a.rows + 31) / 32, static_cast<int64_t>(592), std::max<int64_t>(1, 148 * 16 / blocks)});
     norm_bwd_columns_kernel<TX, TH><<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(parts)), 256, 0, st>>>(a);
     return parts;
 }
@@ -456,7 +862,7 @@ using namespace nvfp4;
 extern "C" int nvfp4_layer_norm(const void* x, int x_dtype, int64_t x_pitch, const void* delta, int delta_dtype, int64_t delta_pitch,
                                 const void* weight, const void* bias, int weight_dtype, float eps, int64_t rows, int64_t cols,
                                 void* sum_out, void* h_out, int h_dtype, float* mean_out, float* rstd_out, float* amax,
-                                nvfp4_stream_t stream) {
+                                int* status, nvfp4_stream_t stream) {
     NVFP4_REQUIRE(x && h_out && (!delta || sum_out) && (mean_out == nullptr) == (rstd_out == nullptr), NVFP4_ERR_ARG, "nvfp4_layer_norm: null pointer");
     NVFP4_REQUIRE(rows > 0 && cols > 0 && cols < (1LL << 30) && x_pitch >= cols && (!delta || delta_pitch >= cols), NVFP4_ERR_ARG,
                   "nvfp4_layer_norm: rows and cols must be positive and the row pitches at least cols");
@@ -466,18 +872,19 @@ extern "C" int nvfp4_layer_norm(const void* x, int x_dtype, int64_t x_pitch, con
                   "nvfp4_layer_norm: the result has the input's type, or BF16 beside an FP32 input");
     NVFP4_REQUIRE(!delta || delta_dtype == x_dtype || (x_dtype == NVFP4_F32 && delta_dtype == NVFP4_BF16), NVFP4_ERR_DTYPE,
                   "nvfp4_layer_norm: the second summand has the input's type, or BF16 beside an FP32 input");
-    NormArgs a{x, delta, weight, bias, sum_out, h_out, mean_out, rstd_out, amax, x_pitch, delta_pitch, rows, static_cast<int>(cols),
+    NormArgs a{x, delta, weight, bias, sum_out, h_out, mean_out, rstd_out, amax, status, x_pitch, delta_pitch, rows, static_cast<int>(cols),
                delta && delta_dtype != x_dtype, weight_dtype, eps};
     // 16-byte vectors of x need every operand's rows to start on a multiple of its own share of them
     const int v = 16 / dtype_size(x_dtype);
     auto fits = [&](const void* p, int dtype, int64_t pitch) { return !p || (aligned(p, std::min(16, v * dtype_size(dtype))) && pitch % v == 0); };
     const bool vector = cols % v == 0 && fits(x, x_dtype, x_pitch) && fits(delta, delta_dtype, delta_pitch) && fits(sum_out, x_dtype, cols) &&
                         fits(h_out, h_dtype, cols) && fits(weight, weight_dtype, 0) && fits(bias, weight_dtype, 0);
+    const bool ring = vector && cols <= 8192 && ring_operand(x, x_dtype, x_pitch, cols) && ring_operand(delta, delta_dtype, delta_pitch, cols);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (x_dtype == NVFP4_BF16) forward<__nv_bfloat16, __nv_bfloat16>(a, vector, st);
-    else if (x_dtype == NVFP4_F16) forward<__half, __half>(a, vector, st);
-    else if (h_dtype == NVFP4_F32) forward<float, float>(a, vector, st);
-    else forward<float, __nv_bfloat16>(a, vector, st);
+    if (x_dtype == NVFP4_BF16) forward<__nv_bfloat16, __nv_bfloat16>(a, vector, ring, st);
+    else if (x_dtype == NVFP4_F16) forward<__half, __half>(a, vector, ring, st);
+    else if (h_dtype == NVFP4_F32) forward<float, float>(a, vector, ring, st);
+    else forward<float, __nv_bfloat16>(a, vector, ring, st);
     return launch_status("nvfp4_layer_norm");
 }
 
@@ -486,34 +893,36 @@ extern "C" int64_t nvfp4_layer_norm_bwd_partials(int64_t rows, int64_t) { return
 extern "C" int nvfp4_layer_norm_bwd(const void* dh, int h_dtype, int64_t dh_pitch, const void* total, int x_dtype, int64_t total_pitch,
                                     const float* mean, const float* rstd, const void* weight, int weight_dtype, const void* dsum,
                                     int64_t dsum_pitch, int64_t rows, int64_t cols, void* dx, void* ddelta, float* partial, void* dweight,
-                                    void* dbias, float* amax, nvfp4_stream_t stream) {
+                                    void* dbias, float* amax, int* status, nvfp4_stream_t stream) {
     NVFP4_REQUIRE(dh && total && mean && rstd && dx && ((!dweight && !dbias) || partial), NVFP4_ERR_ARG, "nvfp4_layer_norm_bwd: null pointer");
     NVFP4_REQUIRE(rows > 0 && cols > 0 && cols < (1LL << 30) && dh_pitch >= cols && total_pitch >= cols && (!dsum || dsum_pitch >= cols), NVFP4_ERR_ARG,
                   "nvfp4_layer_norm_bwd: rows and cols must be positive and the row pitches at least cols");
     NVFP4_REQUIRE(is_float_dtype(x_dtype) && (h_dtype == x_dtype || (x_dtype == NVFP4_F32 && h_dtype == NVFP4_BF16)) &&
                   ((!weight && !dweight && !dbias) || is_float_dtype(weight_dtype)), NVFP4_ERR_DTYPE, "nvfp4_layer_norm_bwd: FP32, BF16 or FP16 tensors");
     NVFP4_REQUIRE(!ddelta || x_dtype == NVFP4_F32, NVFP4_ERR_DTYPE, "nvfp4_layer_norm_bwd: ddelta is the BF16 copy of an FP32 dx");
-    NormBwdArgs a{dh, total, weight, dsum, mean, rstd, dx, ddelta, (dweight || dbias) ? partial : nullptr, amax, dh_pitch, total_pitch, dsum_pitch,
+    NormBwdArgs a{dh, total, weight, dsum, mean, rstd, dx, ddelta, status, (dweight || dbias) ? partial : nullptr, amax, dh_pitch, total_pitch, dsum_pitch,
                   rows, static_cast<int>(cols), weight_dtype};
     const int v = 16 / dtype_size(x_dtype);
     auto fits = [&](const void* p, int dtype, int64_t pitch) { return !p || (aligned(p, std::min(16, v * dtype_size(dtype))) && pitch % v == 0); };
     const bool vector = cols % v == 0 && fits(dh, h_dtype, dh_pitch) && fits(total, x_dtype, total_pitch) && fits(dsum, x_dtype, dsum_pitch) &&
-                        fits(dx, x_dtype, cols) && fits(ddelta, NVFP4_BF16, cols) && fits(weight, weight_dtype, 0);
+                        fits(dx, x_dtype, cols) && fits(ddelta, NVFP4_BF16, cols) && fits(weight, weight_dtype, 0) && aligned(partial, 16);
+    const bool ring = vector && cols <= 8192 && ring_operand(dh, h_dtype, dh_pitch, cols) && ring_operand(total, x_dtype, total_pitch, cols) &&
+                      ring_operand(dsum, x_dtype, dsum_pitch, cols);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     int64_t parts;
-    if (x_dtype == NVFP4_BF16) parts = backward<__nv_bfloat16, __nv_bfloat16>(a, vector, st);
-    else if (x_dtype == NVFP4_F16) parts = backward<__half, __half>(a, vector, st);
-    else if (h_dtype == NVFP4_F32) parts = backward<float, float>(a, vector, st);
-    else parts = backward<float, __nv_bfloat16>(a, vector, st);
+    if (x_dtype == NVFP4_BF16) parts = backward<__nv_bfloat16, __nv_bfloat16>(a, vector, ring, st);
+    else if (x_dtype == NVFP4_F16) parts = backward<__half, __half>(a, vector, ring, st);
+    else if (h_dtype == NVFP4_F32) parts = backward<float, float>(a, vector, ring, st);
+    else parts = backward<float, __nv_bfloat16>(a, vector, ring, st);
     if (a.partial)
-        column_sums_kernel<<<static_cast<unsigned>((2 * cols + 31) / 32), 256, 0, st>>>(partial, parts, 2 * cols, cols, dweight, dbias, weight_dtype);
+        column_sums_kernel<<<static_cast<unsigned>((2 * cols + 31) / 32), 1024, 0, st>>>(partial, parts, 2 * cols, cols, dweight, dbias, weight_dtype);
     return launch_status("nvfp4_layer_norm_bwd");
 }
 
 extern "C" int nvfp4_column_sums(const float* partial, int64_t parts, int64_t cols, void* out, int out_dtype, nvfp4_stream_t stream) {
     NVFP4_REQUIRE(partial && out && parts > 0 && cols > 0 && cols < (1LL << 31), NVFP4_ERR_ARG, "nvfp4_column_sums: null pointer or empty size");
     NVFP4_REQUIRE(is_float_dtype(out_dtype), NVFP4_ERR_DTYPE, "nvfp4_column_sums: FP32, BF16 or FP16 result");
-    column_sums_kernel<<<static_cast<unsigned>((cols + 31) / 32), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+    column_sums_kernel<<<static_cast<unsigned>((cols + 31) / 32), 1024, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
         partial, parts, cols, cols, out, nullptr, out_dtype);
     return launch_status("nvfp4_column_sums");
 }

@@ -22,6 +22,19 @@ template <> __device__ __forceinline__ __half from_float<__half>(float v) { retu
 template <typename T, int V> struct __align__(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Pack { T e[V]; };
 
 template <typename T, int V> __device__ __forceinline__ Pack<T, V> load_pack(const T* p) { return *reinterpret_cast<const Pack<T, V>*>(p); }
+// The same through the read-only path, for tensors that the kernel does not write: such loads may be moved ahead of stores,
+// which a plain load behind a store to an unknown address may not.
+template <typename T, int V> __device__ __forceinline__ Pack<T, V> load_const(const T* p) {
+    Pack<T, V> v;
+    if constexpr (sizeof(v) == 32) {
+        reinterpret_cast<uint4*>(&v)[0] = __ldg(reinterpret_cast<const uint4*>(p));
+        reinterpret_cast<uint4*>(&v)[1] = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+    } else if constexpr (sizeof(v) == 16) *reinterpret_cast<uint4*>(&v) = __ldg(reinterpret_cast<const uint4*>(p));
+    else if constexpr (sizeof(v) == 8) *reinterpret_cast<uint2*>(&v) = __ldg(reinterpret_cast<const uint2*>(p));
+    else if constexpr (sizeof(v) == 4) *reinterpret_cast<uint32_t*>(&v) = __ldg(reinterpret_cast<const uint32_t*>(p));
+    else *reinterpret_cast<uint16_t*>(&v) = __ldg(reinterpret_cast<const uint16_t*>(p));
+    return v;
+}
 template <typename T, int V> __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v) { *reinterpret_cast<Pack<T, V>*>(p) = v; }
 template <typename T, int V> __device__ __forceinline__ void unpack(const Pack<T, V>& v, float (&f)[V]) {
 #pragma unroll
@@ -41,9 +54,9 @@ template <typename T, int V> __device__ __forceinline__ float abs_max(const Pack
 }
 // V parameters (weight, bias) of a type known at run time; the branch is the same for the whole grid
 template <int V> __device__ __forceinline__ void load_param(const void* p, int dtype, int64_t i, float (&f)[V]) {
-    if (dtype == NVFP4_F32) unpack(load_pack<float, V>(static_cast<const float*>(p) + i), f);
-    else if (dtype == NVFP4_BF16) unpack(load_pack<__nv_bfloat16, V>(static_cast<const __nv_bfloat16*>(p) + i), f);
-    else unpack(load_pack<__half, V>(static_cast<const __half*>(p) + i), f);
+    if (dtype == NVFP4_F32) unpack(load_const<float, V>(static_cast<const float*>(p) + i), f);
+    else if (dtype == NVFP4_BF16) unpack(load_const<__nv_bfloat16, V>(static_cast<const __nv_bfloat16*>(p) + i), f);
+    else unpack(load_const<__half, V>(static_cast<const __half*>(p) + i), f);
 }
 __device__ __forceinline__ void store_param(void* p, int dtype, int64_t i, float v) {
     if (dtype == NVFP4_F32) static_cast<float*>(p)[i] = v;

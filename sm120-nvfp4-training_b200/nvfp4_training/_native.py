@@ -49,9 +49,9 @@ _SIGNATURES = {
     "nvfp4_rmsnorm_bwd": (I32, [P, P, P, P, P, I64, I64, P, P, P, P, P]),
     "nvfp4_cross_entropy_fwd": (I32, [P, I64, P, I64, I64, P, P, P, P]),
     "nvfp4_cross_entropy_bwd": (I32, [P, I64, P, P, P, I64, I64, P, I64, P, P]),
-    "nvfp4_layer_norm": (I32, [P, I32, I64, P, I32, I64, P, P, I32, F, I64, I64, P, P, I32, P, P, P, P]),
+    "nvfp4_layer_norm": (I32, [P, I32, I64, P, I32, I64, P, P, I32, F, I64, I64, P, P, I32, P, P, P, P, P]),
     "nvfp4_layer_norm_bwd_partials": (I64, [I64, I64]),
-    "nvfp4_layer_norm_bwd": (I32, [P, I32, I64, P, I32, I64, P, P, P, I32, P, I64, I64, I64, P, P, P, P, P, P, P]),
+    "nvfp4_layer_norm_bwd": (I32, [P, I32, I64, P, I32, I64, P, P, P, I32, P, I64, I64, I64, P, P, P, P, P, P, P, P]),
     "nvfp4_fp8_quantize": (I32, [P, I32, I64, I64, I64, I32, P, P, P, P, P, P]),
     "nvfp4_fp8_gemm": (I32, [P, P, P, P, I64, I64, I64, P, I32, P, I32, I64, P, P]),
     "nvfp4_column_sums": (I32, [P, I64, I64, P, I32, P]),

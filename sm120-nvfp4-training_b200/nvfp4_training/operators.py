@@ -70,7 +70,8 @@ def _norm_forward(x, delta, weight, bias, eps, out_dtype, amax, keep_stats):
             nat.check(nat.lib().nvfp4_layer_norm(
                 x2.data_ptr(), codes[x.dtype], pitch_of(x2), nat.ptr(d2), 0 if d2 is None else codes[d2.dtype], 0 if d2 is None else pitch_of(d2),
                 nat.ptr(weight), nat.ptr(bias), 0 if affine is None else codes[affine.dtype], eps, rows, cols,
-                None if d2 is None else total.data_ptr(), h.data_ptr(), codes[out_dtype], at, at and at + 4 * rows, nat.ptr(amax), nat.raw_stream(dev)))
+                None if d2 is None else total.data_ptr(), h.data_ptr(), codes[out_dtype], at, at and at + 4 * rows, nat.ptr(amax),
+                nat.status_word(dev).data_ptr(), nat.raw_stream(dev)))
     return total, h, stats
 
 
@@ -117,7 +118,8 @@ class _LayerNorm(torch.autograd.Function):
                 nat.check(lib.nvfp4_layer_norm_bwd(
                     g.data_ptr(), codes[g.dtype], pitch_of(g), total.data_ptr(), codes[total.dtype], pitch_of(total), at, at + 4 * rows,
                     nat.ptr(weight), 0 if wdtype is None else codes[wdtype], nat.ptr(res), 0 if res is None else pitch_of(res), rows, cols,
-                    dx.data_ptr(), nat.ptr(dd), nat.ptr(partial), nat.ptr(dw), nat.ptr(db), nat.ptr(amax), nat.raw_stream(dev)))
+                    dx.data_ptr(), nat.ptr(dd), nat.ptr(partial), nat.ptr(dw), nat.ptr(db), nat.ptr(amax),
+                    nat.status_word(dev).data_ptr(), nat.raw_stream(dev)))
         else:
             for t in (dw, db):
                 if t is not None:

@@ -78,12 +78,12 @@ def test_entry_points_refuse_before_any_launch():
     buf = C.create_string_buffer(4096)
 
     def norm(x=buf, xd=1, pitch=8, delta=None, dd=1, eps=1e-5, rows=4, cols=8, total=None, h=buf, hd=1, mean=None, rstd=None):
-        return lib.nvfp4_layer_norm(x, xd, pitch, delta, dd, 8, None, None, 0, eps, rows, cols, total, h, hd, mean, rstd, None, None)
+        return lib.nvfp4_layer_norm(x, xd, pitch, delta, dd, 8, None, None, 0, eps, rows, cols, total, h, hd, mean, rstd, None, None, None)
     assert norm(x=None) == 1 and norm(h=None) == 1 and norm(delta=buf) == 1 and norm(mean=buf) == 1
     assert norm(rows=0) == 1 and norm(cols=0) == 1 and norm(pitch=7) == 1
     assert norm(xd=3) == 3 and norm(hd=0) == 3 and norm(xd=0, hd=2) == 3 and norm(delta=buf, total=buf, dd=2) == 3
     bwd = lambda dd=None, dw=None, part=None, xd=1, hd=1: lib.nvfp4_layer_norm_bwd(buf, hd, 8, buf, xd, 8, buf, buf, None, 0, None, 0, 4, 8, buf, dd,
-                                                                                 part, dw, None, None, None)
+                                                                                 part, dw, None, None, None, None)
     assert bwd(dw=buf) == 1 and bwd(dd=buf) == 3 and bwd(xd=2, hd=1) == 3
     assert lib.nvfp4_layer_norm_bwd_partials(1, 8) == 1 and lib.nvfp4_layer_norm_bwd_partials(10 ** 9, 8) <= 1024
 
