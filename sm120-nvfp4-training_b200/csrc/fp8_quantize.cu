@@ -51,7 +51,7 @@ template <typename T> struct Fp8Map {
 
 // Magnitude maxima as integers: 16-bit types two to a register, FP32 one.
 template <typename T> struct Magnitude {
-    static constexpr int PER = sizeof(T) == 2 ? 2 : 1, WORDS = 4;      // per register; registers per 16-byte vector
+    static constexpr int PER = sizeof(T) == 2 ? 2 : 1;                 // per register
     static __device__ __forceinline__ uint32_t of(uint32_t w) { return w & (PER == 2 ? 0x7fff7fffu : 0x7fffffffu); }
     static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return PER == 2 ? __vmaxu2(a, b) : max(a, b); }
     static __device__ __forceinline__ uint32_t single(uint32_t m) { return PER == 2 ? max(m & 0xffffu, m >> 16) : m; }      // of a register's two
@@ -61,7 +61,6 @@ template <typename T> struct Magnitude {
         else return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
     }
 };
-template <typename T, int E> __device__ __forceinline__ const uint32_t* words(const Pack<T, E>& v) { return reinterpret_cast<const uint32_t*>(&v); }
 
 template <typename T, bool COL, bool SQUARE>
 __global__ void __launch_bounds__(F8_THREADS, Fp8Map<T>::CTAS) fp8_quantize_kernel(const Fp8Args a) {
@@ -88,15 +87,14 @@ __global__ void __launch_bounds__(F8_THREADS, Fp8Map<T>::CTAS) fp8_quantize_kern
             else {
 #pragma unroll
                 for (int j = 0; j < E; ++j)
-                    if (col0 + j < a.cols) v[i].e[j] = src[i * a.pitch + j];
+                    if (col0 + j < a.cols) set_element(v[i], j, src[i * a.pitch + j]);
             }
         }
     }
     uint32_t row_best[I];
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-        const uint32_t* w = words(v[i]);
-        row_best[i] = Mag::larger(Mag::larger(Mag::of(w[0]), Mag::of(w[1])), Mag::larger(Mag::of(w[2]), Mag::of(w[3])));
+        row_best[i] = Mag::larger(Mag::larger(Mag::of(v[i].w[0]), Mag::of(v[i].w[1])), Mag::larger(Mag::of(v[i].w[2]), Mag::of(v[i].w[3])));
     }
     Fp8Scale square{};
     if constexpr (SQUARE) {
@@ -140,7 +138,7 @@ __global__ void __launch_bounds__(F8_THREADS, Fp8Map<T>::CTAS) fp8_quantize_kern
         for (int j = 0; j < E; ++j) {
             float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < I; ++i) sum += to_float(v[i].e[j]);
+            for (int i = 0; i < I; ++i) sum += element(v[i], j);
             if (L == 16) sum += __shfl_xor_sync(0xffffffffu, sum, 16);
             if (part == 0) warp_cols[warp][col_in + j] = sum;
         }
@@ -156,9 +154,9 @@ __global__ void __launch_bounds__(F8_THREADS, Fp8Map<T>::CTAS) fp8_quantize_kern
     if constexpr (COL && !SQUARE) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            uint32_t best = Mag::of(words(v[0])[k]);
+            uint32_t best = Mag::of(v[0].w[k]);
 #pragma unroll
-            for (int i = 1; i < I; ++i) best = Mag::larger(best, Mag::of(words(v[i])[k]));
+            for (int i = 1; i < I; ++i) best = Mag::larger(best, Mag::of(v[i].w[k]));
             if (L == 16) best = Mag::larger(best, __shfl_xor_sync(0xffffffffu, best, 16));
             if (part == 0) {
                 if constexpr (Mag::PER == 2) {
@@ -210,7 +208,7 @@ __global__ void __launch_bounds__(F8_THREADS, Fp8Map<T>::CTAS) fp8_quantize_kern
             for (int p = 0; p < I / 8; ++p) {
                 float f[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) f[i] = to_float(v[p * 8 + i].e[j]) * inv;
+                for (int i = 0; i < 8; ++i) f[i] = element(v[p * 8 + i], j) * inv;
                 const int piece = (row_in >> 3) + p;
                 *reinterpret_cast<uint2*>(turned + c * 128 + ((piece ^ (c >> 3)) & 15) * 8) =
                     make_uint2(e4m3x4(f[0], f[1], f[2], f[3]), e4m3x4(f[4], f[5], f[6], f[7]));
