@@ -393,9 +393,9 @@ __global__ void __launch_bounds__(1024) column_sums_kernel(const float* __restri
 // With its operands in registers alone a CTA loads a row, waits, reduces, waits, and stores: 0.3 to 0.6 of HBM, all of it load
 // latency (long-scoreboard stalls 10 of 16 cycles per instruction).  Here one thread keeps bulk copies of the next rows in
 // flight into a ring of stages, and a stage is refilled as soon as the CTA's first barrier behind its reads has passed.  CTAs
-// are persistent, so weight and bias (and the backward pass's column sums) stay in registers: eight columns per thread, as
-// one 16-byte vector of a 16-bit x or two of an FP32 one, up to 8192 columns.  Narrow rows have several groups of threads side
-// by side in a CTA; R rows of each group share the barriers of a round.
+// are persistent, so weight and bias (and the backward pass's column sums) stay in registers: C columns per thread as 16-byte
+// vectors of x, up to 8192 columns.  Narrow rows have several groups of threads side by side in a CTA; R rows of each group
+// share the barriers of a round.
 namespace ring {
 constexpr int MAX_STAGES = 8;
 constexpr int BYTES_PER_SM = 216 * 1024;
@@ -503,11 +503,11 @@ template <typename T, int V> __device__ __forceinline__ void load_or(const void*
     if (p && live) load_param<V>(p, dtype, c, f);
 }
 
-template <typename TX, typename TD, typename TO, int R, int MAXT>
-__global__ void __launch_bounds__(MAXT, MAXT == 256 ? 4 : MAXT == 640 ? 2 : 1) norm_fwd_ring_kernel(const NormArgs a, int stages, int row_threads) {
-    constexpr int V = 16 / sizeof(TX), N = 8 / V;
+template <typename TX, typename TD, typename TO, int C, int R, int MAXT, int CTAS>
+__global__ void __launch_bounds__(MAXT, CTAS) norm_fwd_ring_kernel(const NormArgs a, int stages, int row_threads) {
+    constexpr int V = 16 / sizeof(TX), N = C / V;
     extern __shared__ __align__(128) uint8_t ring_data[];
-    __shared__ float slots[2][32][R];
+    __shared__ float2 slots[2][R][32];           // a warp's sum and its squares around its own mean
     __shared__ RowRing<2> q;
     const int group = threadIdx.x / row_threads, tid = threadIdx.x - group * row_threads, step = row_threads, vectors = a.cols / V;
     const int per_stage = blockDim.x / row_threads * R, first_warp = group * (row_threads >> 5);
@@ -531,9 +531,20 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 4 : MAXT == 640 ? 2 : 1) n
         load_or(a.weight, a.weight_dtype, c * V, c < vectors, 1.f, w[i]);
         load_or(a.bias, a.weight_dtype, c * V, c < vectors, 0.f, b[i]);
     }
+    // columns of this warp, and of warp `lane` of the group (what the gather below needs)
+    const int lane = threadIdx.x & 31, warps = step >> 5;
+    float mine = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) mine += tid + i * step < vectors ? static_cast<float>(V) : 0.f;
+    mine = warp_sum(mine);
+    if (lane == 0) slots[0][0][threadIdx.x >> 5].x = mine;
+    __syncthreads();
+    const float theirs = lane < warps ? slots[0][0][first_warp + lane].x : 0.f;
+    const float inv_mine = mine > 0.f ? 1.f / mine : 0.f, inv_theirs = theirs > 0.f ? 1.f / theirs : 0.f;
+    int half = 1;
     const float inv_n = 1.f / static_cast<float>(a.cols);
     float best = 0.f;
-    for (int64_t g = blockIdx.x; g < runs; g += gridDim.x) {
+    for (int64_t g = blockIdx.x; g < runs; g += gridDim.x, half ^= 1) {
         aop::mbar_wait(&q.full[at.slot], at.phase, &q.abort_flag);
         const uint8_t* stage = ring_data + at.slot * stage_bytes;
         float f[R][N][V], sums[R];
@@ -559,26 +570,48 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 4 : MAXT == 640 ? 2 : 1) n
                 for (int j = 0; j < V; ++j) sums[k] += f[k][i][j];
             }
         }
-        group_sums(sums, slots[0], first_warp, step >> 5);
-        ring_advance(q, ring_data, at, stages, g);
-        float mean[R];
+        // the warp's mean and squares around it, then the group's from the warps': one barrier, no cancellation
+        float squares[R], mean[R];
+#pragma unroll
+        for (int k = 0; k < R; ++k) sums[k] = warp_sum(sums[k]);
 #pragma unroll
         for (int k = 0; k < R; ++k) {
-            mean[k] = sums[k] * inv_n;
-            sums[k] = 0.f;
+            const float m = sums[k] * inv_mine;
+            squares[k] = 0.f;
 #pragma unroll
             for (int i = 0; i < N; ++i)
                 if (tid + i * step < vectors) {
 #pragma unroll
-                    for (int j = 0; j < V; ++j) { const float d = f[k][i][j] - mean[k]; sums[k] = fmaf(d, d, sums[k]); }
+                    for (int j = 0; j < V; ++j) { const float d = f[k][i][j] - m; squares[k] = fmaf(d, d, squares[k]); }
                 }
         }
-        group_sums(sums, slots[1], first_warp, step >> 5);
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            squares[k] = warp_sum(squares[k]);
+            if (lane == 0) slots[half][k][threadIdx.x >> 5] = make_float2(sums[k], squares[k]);
+        }
+        __syncthreads();
+        ring_advance(q, ring_data, at, stages, g);
+        if (warps > 1) {
+            float2 part[R];
+#pragma unroll
+            for (int k = 0; k < R; ++k) {
+                part[k] = lane < warps ? slots[half][k][first_warp + lane] : make_float2(0.f, 0.f);
+                sums[k] = warp_sum(part[k].x);
+            }
+#pragma unroll
+            for (int k = 0; k < R; ++k) {
+                const float d = part[k].x * inv_theirs - sums[k] * inv_n;
+                squares[k] = warp_sum(fmaf(theirs * d, d, part[k].y));
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < R; ++k) mean[k] = sums[k] * inv_n;
 #pragma unroll
         for (int k = 0; k < R; ++k) {
             const int64_t r = g * per_stage + group * R + k;
             if (r >= a.rows) continue;
-            const float rstd = rsqrtf(sums[k] * inv_n + a.eps);
+            const float rstd = rsqrtf(squares[k] * inv_n + a.eps);
             if (tid == 0 && a.mean) { a.mean[r] = mean[k]; a.rstd[r] = rstd; }
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -597,9 +630,9 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 4 : MAXT == 640 ? 2 : 1) n
     ring_finish(q, a.status);
 }
 
-template <typename TX, typename TH, int R, int MAXT>
-__global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) norm_bwd_ring_kernel(const NormBwdArgs a, int stages, int row_threads) {
-    constexpr int V = 16 / sizeof(TX), N = 8 / V;
+template <typename TX, typename TH, int C, int R, int MAXT, int CTAS>
+__global__ void __launch_bounds__(MAXT, CTAS) norm_bwd_ring_kernel(const NormBwdArgs a, int stages, int row_threads) {
+    constexpr int V = 16 / sizeof(TX), N = C / V;
     extern __shared__ __align__(128) uint8_t ring_data[];
     __shared__ float slots[2][32][2 * R];
     __shared__ RowRing<3> q;
@@ -712,12 +745,15 @@ constexpr int64_t MAX_GRID = 1 << 30;
 
 static int round32(int n) { return (n + 31) / 32 * 32; }
 
-// Threads for eight columns each, narrow rows in groups that make 256 threads; as many CTAs per SM as give about 1024 threads
-// and leave each of them three stages.
-static int row_threads_for(int64_t cols) { return round32(static_cast<int>((cols + 7) / 8)); }
+// Sixteen columns a thread from 2048 columns on, eight below: a round costs a thread about 150 instructions whatever it holds
+// (waiting, two reductions, addresses), which sixteen columns halve (16384 x 5120 BF16: 179 -> FWD us forward, 165 -> BWD
+// backward); below, the rows would not fill a warp.  Narrow rows stand in groups that make 256 threads.  As many CTAs per SM
+// as the registers allow and as leave each of them three stages.
+static int columns_per_thread(int64_t cols) { return cols >= 2048 ? 16 : 8; }
 static ring::Plan ring_plan(int64_t rows, int64_t cols, int rows_per_group, int row_bytes, int sms, int threads_per_sm, bool backward) {
     ring::Plan p;
-    p.row_threads = row_threads_for(cols);
+    const int per_thread = columns_per_thread(cols);
+    p.row_threads = round32(static_cast<int>((cols + per_thread - 1) / per_thread));
     // few rows: no group without one
     const int64_t want = std::max<int64_t>(1, (rows + static_cast<int64_t>(rows_per_group) * sms - 1) / (static_cast<int64_t>(rows_per_group) * sms));
     const int groups = static_cast<int>(std::min<int64_t>(std::max(1, 256 / p.row_threads), want));
@@ -725,7 +761,7 @@ static ring::Plan ring_plan(int64_t rows, int64_t cols, int rows_per_group, int 
     p.stage_bytes = groups * rows_per_group * row_bytes;
     p.ctas = std::max(1, std::min(threads_per_sm / p.threads, ring::BYTES_PER_SM / (3 * p.stage_bytes + 2048)));
     p.stages = std::max(2, std::min(ring::MAX_STAGES, (ring::BYTES_PER_SM / p.ctas - 2048) / p.stage_bytes));
-    // the groups' column sums of the backward pass (8 bytes a column) fit the stages: a row alone is 4 bytes a column or more
+    // the groups' column sums of the backward pass (8 bytes a column) meet in the stages
     if (backward) while (p.stages * p.stage_bytes < groups * 8 * cols) ++p.stages;
     const int64_t all = (rows + static_cast<int64_t>(groups) * rows_per_group - 1) / (static_cast<int64_t>(groups) * rows_per_group);
     p.ctas = static_cast<int>(std::min<int64_t>({all, static_cast<int64_t>(p.ctas) * sms, NORM_MAX_PARTS}));
@@ -755,36 +791,33 @@ static bool launch_ring(void (*kernel)(Args, int, int), bool (&ready)[64], const
     kernel<<<p.ctas, p.threads, p.stages * p.stage_bytes, st>>>(a, p.stages, p.row_threads);
     return true;
 }
-template <typename TX, typename TD, typename TO, int R, int MAXT>
+template <typename TX, typename TD, typename TO, int C, int R, int MAXT, int CTAS>
 static bool fwd_ring(const NormArgs& a, const ring::Plan& p, cudaStream_t st) {
     static bool ready[64] = {};
-    return launch_ring<NormArgs>(norm_fwd_ring_kernel<TX, TD, TO, R, MAXT>, ready, a, p, st);
+    return launch_ring<NormArgs>(norm_fwd_ring_kernel<TX, TD, TO, C, R, MAXT, CTAS>, ready, a, p, st);
 }
 template <typename TX, typename TD, typename TO>
 static bool fwd_ring_sized(const NormArgs& a, cudaStream_t st) {
     const int row_bytes = a.cols * static_cast<int>(sizeof(TX) + (a.delta ? sizeof(TD) : 0));
-    // two rows a round where the rows are short; above 256 threads one, in two CTAs of up to 48 registers a thread
-    const int threads = row_threads_for(a.cols), r = threads <= 256 ? 2 : 1;
-    const ring::Plan p = ring_plan(a.rows, a.cols, r, row_bytes, sm_count(), r == 2 ? 1024 : 1344, false);
-    if (threads <= 256) return fwd_ring<TX, TD, TO, 2, 256>(a, p, st);
-    if (threads <= 640) return fwd_ring<TX, TD, TO, 1, 640>(a, p, st);
-    return fwd_ring<TX, TD, TO, 1, 1024>(a, p, st);
+    if (columns_per_thread(a.cols) == 8)
+        return fwd_ring<TX, TD, TO, 8, 2, 256, 4>(a, ring_plan(a.rows, a.cols, 2, row_bytes, sm_count(), 1024, false), st);
+    const ring::Plan p = ring_plan(a.rows, a.cols, 1, row_bytes, sm_count(), 640, false);
+    if (p.threads <= 256) return fwd_ring<TX, TD, TO, 16, 1, 256, 2>(a, p, st);
+    return p.threads <= 320 ? fwd_ring<TX, TD, TO, 16, 1, 320, 2>(a, p, st) : fwd_ring<TX, TD, TO, 16, 1, 512, 1>(a, p, st);
 }
-template <typename TX, typename TH, int R, int MAXT>
+template <typename TX, typename TH, int C, int R, int MAXT, int CTAS>
 static int64_t bwd_ring(const NormBwdArgs& a, const ring::Plan& p, cudaStream_t st) {
     static bool ready[64] = {};
-    return launch_ring<NormBwdArgs>(norm_bwd_ring_kernel<TX, TH, R, MAXT>, ready, a, p, st) ? p.ctas : 0;
+    return launch_ring<NormBwdArgs>(norm_bwd_ring_kernel<TX, TH, C, R, MAXT, CTAS>, ready, a, p, st) ? p.ctas : 0;
 }
 template <typename TX, typename TH>
 static int64_t bwd_ring_sized(const NormBwdArgs& a, cudaStream_t st) {
     const int row_bytes = a.cols * static_cast<int>(sizeof(TH) + sizeof(TX) * (a.dsum ? 2 : 1));
-    // two rows a round where two stages of two rows fit
-    const int threads = row_threads_for(a.cols), r = threads <= 768 && 4 * row_bytes <= ring::BYTES_PER_SM - 2048 ? 2 : 1;
-    const ring::Plan p = ring_plan(a.rows, a.cols, r, row_bytes, sm_count(), 1024, true);
-    if (r == 1) return bwd_ring<TX, TH, 1, 1024>(a, p, st);
-    if (threads <= 256) return bwd_ring<TX, TH, 2, 256>(a, p, st);
-    if (threads <= 512) return bwd_ring<TX, TH, 2, 512>(a, p, st);
-    return bwd_ring<TX, TH, 2, 768>(a, p, st);
+    if (columns_per_thread(a.cols) == 8)
+        return bwd_ring<TX, TH, 8, 2, 256, 2>(a, ring_plan(a.rows, a.cols, 2, row_bytes, sm_count(), 512, true), st);
+    const ring::Plan p = ring_plan(a.rows, a.cols, 1, row_bytes, sm_count(), 640, true);
+    if (p.threads <= 256) return bwd_ring<TX, TH, 16, 1, 256, 2>(a, p, st);
+    return p.threads <= 320 ? bwd_ring<TX, TH, 16, 1, 320, 2>(a, p, st) : bwd_ring<TX, TH, 16, 1, 512, 1>(a, p, st);
 }
 
 template <typename TX, typename TO, int V>
