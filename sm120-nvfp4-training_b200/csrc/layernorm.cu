@@ -398,8 +398,8 @@ __global__ void __launch_bounds__(1024) column_sums_kernel(const float* __restri
 // share the barriers of a round.
 namespace ring {
 constexpr int MAX_STAGES = 8;
-constexpr int BYTES_PER_SM = 216 * 1024;
-struct Plan { int row_threads, threads, stages, stage_bytes, ctas; };
+constexpr int BYTES_PER_SM = 228 * 1024, ASIDE = 2560;      // of it a CTA's own 1024 bytes and its static arrays
+struct Plan { int row_threads, threads, stages, stage_bytes, ctas, parked; };      // parked: bytes behind the stages
 }  // namespace ring
 
 struct RingOperand { const uint8_t* base; int64_t pitch; uint32_t bytes; };       // pitch and row length in bytes; base null: absent
@@ -630,6 +630,12 @@ __global__ void __launch_bounds__(MAXT, CTAS) norm_fwd_ring_kernel(const NormArg
     ring_finish(q, a.status);
 }
 
+__device__ __forceinline__ float4 shared_again(const float4* p) {      // a load that stays where it is written
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(aop::smem_u32(p)));
+    return v;
+}
+
 template <typename TX, typename TH, int C, int R, int MAXT, int CTAS>
 __global__ void __launch_bounds__(MAXT, CTAS) norm_bwd_ring_kernel(const NormBwdArgs a, int stages, int row_threads) {
     constexpr int V = 16 / sizeof(TX), N = C / V;
@@ -652,12 +658,19 @@ __global__ void __launch_bounds__(MAXT, CTAS) norm_bwd_ring_kernel(const NormBwd
     const int64_t runs = q.groups;
     const uint32_t stage_bytes = per_stage * q.row_bytes;
     RingCursor at{0, 0};
+    // With sixteen columns a thread keeps its weights in shared memory, in registers they would spill.
+    constexpr bool PARKED = C == 16;
     float w[N][V], acc_w[N][V], acc_b[N][V];
+    float4* parked = reinterpret_cast<float4*>(ring_data + stages * stage_bytes) + threadIdx.x;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         load_or(a.weight, a.weight_dtype, (tid + i * step) * V, tid + i * step < vectors, 1.f, w[i]);
 #pragma unroll
         for (int j = 0; j < V; ++j) acc_w[i][j] = acc_b[i][j] = 0.f;
+        if constexpr (PARKED) {
+#pragma unroll
+            for (int j = 0; j < V; j += 4) parked[(i * V + j) / 4 * blockDim.x] = make_float4(w[i][j], w[i][j + 1], w[i][j + 2], w[i][j + 3]);
+        }
     }
     const float inv_n = 1.f / static_cast<float>(a.cols);
     float best = 0.f, mean[R], rstd[R];          // of the next group, fetched one round ahead
@@ -687,6 +700,13 @@ __global__ void __launch_bounds__(MAXT, CTAS) norm_bwd_ring_kernel(const NormBwd
                 if (c >= vectors || g * per_stage + row >= a.rows) continue;
                 unpack(load_pack<TH, V>(reinterpret_cast<const TH*>(stage + row * h_bytes) + c * V), u[k][i]);
                 unpack(load_pack<TX, V>(reinterpret_cast<const TX*>(stage + per_stage * h_bytes + row * x_bytes) + c * V), z[k][i]);
+                if constexpr (PARKED) {
+#pragma unroll
+                    for (int j = 0; j < V; j += 4) {
+                        const float4 t = shared_again(parked + (i * V + j) / 4 * blockDim.x);
+                        w[i][j] = t.x; w[i][j + 1] = t.y; w[i][j + 2] = t.z; w[i][j + 3] = t.w;
+                    }
+                }
                 if (a.dsum) res[k][i] = load_pack<TX, V>(reinterpret_cast<const TX*>(stage + per_stage * (h_bytes + x_bytes) + row * s_bytes) + c * V);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
@@ -746,7 +766,7 @@ constexpr int64_t MAX_GRID = 1 << 30;
 static int round32(int n) { return (n + 31) / 32 * 32; }
 
 // Sixteen columns a thread from 2048 columns on, eight below: a round costs a thread about 150 instructions whatever it holds
-// (waiting, two reductions, addresses), which sixteen columns halve (16384 x 5120 BF16: 179 -> FWD us forward, 165 -> BWD
+// (waiting, two reductions, addresses), which sixteen columns halve (16384 x 5120 BF16: 179 -> 109 us forward, 165 -> 137
 // backward); below, the rows would not fill a warp.  Narrow rows stand in groups that make 256 threads.  As many CTAs per SM
 // as the registers allow and as leave each of them three stages.
 static int columns_per_thread(int64_t cols) { return cols >= 2048 ? 16 : 8; }
@@ -759,8 +779,10 @@ static ring::Plan ring_plan(int64_t rows, int64_t cols, int rows_per_group, int 
     const int groups = static_cast<int>(std::min<int64_t>(std::max(1, 256 / p.row_threads), want));
     p.threads = p.row_threads * groups;
     p.stage_bytes = groups * rows_per_group * row_bytes;
-    p.ctas = std::max(1, std::min(threads_per_sm / p.threads, ring::BYTES_PER_SM / (3 * p.stage_bytes + 2048)));
-    p.stages = std::max(2, std::min(ring::MAX_STAGES, (ring::BYTES_PER_SM / p.ctas - 2048) / p.stage_bytes));
+    p.parked = backward && per_thread == 16 ? p.threads * 16 * 4 : 0;
+    const int aside = p.parked + ring::ASIDE;
+    p.ctas = std::max(1, std::min(threads_per_sm / p.threads, ring::BYTES_PER_SM / (3 * p.stage_bytes + aside)));
+    p.stages = std::max(2, std::min(ring::MAX_STAGES, (ring::BYTES_PER_SM / p.ctas - aside) / p.stage_bytes));
     // the groups' column sums of the backward pass (8 bytes a column) meet in the stages
     if (backward) while (p.stages * p.stage_bytes < groups * 8 * cols) ++p.stages;
     const int64_t all = (rows + static_cast<int64_t>(groups) * rows_per_group - 1) / (static_cast<int64_t>(groups) * rows_per_group);
@@ -785,10 +807,10 @@ static bool launch_ring(void (*kernel)(Args, int, int), bool (&ready)[64], const
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) return false;
     if (!ready[dev]) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring::BYTES_PER_SM) != cudaSuccess) return false;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring::BYTES_PER_SM - ring::ASIDE) != cudaSuccess) return false;
         ready[dev] = true;
     }
-    kernel<<<p.ctas, p.threads, p.stages * p.stage_bytes, st>>>(a, p.stages, p.row_threads);
+    kernel<<<p.ctas, p.threads, p.stages * p.stage_bytes + p.parked, st>>>(a, p.stages, p.row_threads);
     return true;
 }
 template <typename TX, typename TD, typename TO, int C, int R, int MAXT, int CTAS>

@@ -245,3 +245,24 @@ def test_module_under_autocast_hands_its_amax_on():
     assert x.grad is not None and norm.weight.grad.dtype == F32
     plain = torch.nn.LayerNorm(320, elementwise_affine=False)
     assert nv.LayerNorm(320, elementwise_affine=False)(x).shape == plain(x).shape
+
+
+@pytest.mark.parametrize("cols", [16, 64, 1024, 2040, 2048, 4096, 6144, 8184, 8192, 8200])
+@pytest.mark.parametrize("rows", [1, 3, 700])
+@pytest.mark.parametrize("dtype,delta_dtype", [(BF16, BF16), (F32, BF16), (F32, F32)])
+def test_widths_around_the_kernels_borders(cols, rows, dtype, delta_dtype):
+    """Few and many rows on both sides of each width at which the work is divided differently (tolerances as above)."""
+    g = torch.Generator(device="cuda").manual_seed(cols + rows)
+    x, d = rand(g, rows, cols, dtype=dtype).requires_grad_(True), rand(g, rows, cols, dtype=delta_dtype).requires_grad_(True)
+    w, b = (1 + 0.2 * rand(g, cols)).requires_grad_(True), rand(g, cols).requires_grad_(True)
+    dh, ds = rand(g, rows, cols, dtype=dtype), rand(g, rows, cols, dtype=dtype)
+    total, h = nv.add_layer_norm(x, d, w, b)
+    grads = torch.autograd.grad((h, total), (x, d, w, b), (dh, ds))
+    want, z, rstd = reference(total.detach(), w.detach(), b.detach(), 1e-5)
+    check(h, want, 8.0, "h")
+    wdx, wdw, wdb, u = gradients(z, rstd, w.detach(), dh, ds)
+    size = (rstd * u.abs().max(-1, keepdim=True).values).max().item() * max(1.0, z.abs().max().item()) ** 2 + 1
+    for got, want, scale in zip(grads, (wdx, wdx, wdw, wdb), (8 * size, 8 * size, 8 * dh.abs().max().item() * rows, dh.abs().max().item() * rows)):
+        check(got, want, scale, "gradients")
+    from nvfp4_training import _native
+    _native.check_status()
