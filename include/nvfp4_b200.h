@@ -398,6 +398,24 @@ int nvfp4_fp8_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* b, 
                    nvfp4_stream_t stream);
 int nvfp4_column_sums(const float* partial, int64_t parts, int64_t cols, void* out, int out_dtype, nvfp4_stream_t stream);
 
+/*
+ * The linear layer whole, as one call each way.  A packing of [rows][k] is its codes followed by its scale blocks, 16-byte
+ * aligned: nvfp4_fp8_packing_bytes(rows, k) bytes.
+ * nvfp4_fp8_linear: y[m][n] = Q(x) Q(w)^T (+ bias).  w [n][k] of w_dtype, quantised in the call, or with w_dtype NVFP4_E4M3 its
+ *   packing (w_pitch unused).  x_t, w_t (nullable): the transposed packings [k][m] and [k][n] that the backward pass reads.
+ *   work: nvfp4_fp8_packing_bytes(m, k) bytes, and as many for [n][k] where w is quantised.
+ * nvfp4_fp8_linear_bwd: dx[m][k] = Q(dy) Q(w), dw[n][k] = Q'(dy)^T Q'(x), dbias[n] = sum of dy; each nullable (dx needs w_t, dw
+ *   needs x_t).  work: nvfp4_fp8_packing_bytes(m, n) where dx is asked for, nvfp4_fp8_packing_bytes(n, m) and 4 * n *
+ *   ceil(m / 128) bytes where dw or dbias is.
+ */
+int64_t nvfp4_fp8_packing_bytes(int64_t rows, int64_t k);
+int nvfp4_fp8_linear(const void* x, int x_dtype, int64_t m, int64_t k, int64_t x_pitch, const void* w, int w_dtype, int64_t n,
+                     int64_t w_pitch, const void* bias, int bias_dtype, void* y, uint8_t* work, uint8_t* x_t, uint8_t* w_t,
+                     int* status, nvfp4_stream_t stream);
+int nvfp4_fp8_linear_bwd(const void* dy, int dtype, int64_t m, int64_t n, int64_t k, int64_t dy_pitch, const uint8_t* x_t,
+                         const uint8_t* w_t, void* dx, void* dw, int dw_dtype, void* dbias, int dbias_dtype, uint8_t* work,
+                         int* status, nvfp4_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

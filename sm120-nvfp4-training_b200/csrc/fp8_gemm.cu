@@ -51,6 +51,12 @@ __device__ __forceinline__ void mma8(uint32_t tmem_d, uint64_t desc_a, uint64_t 
             "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
             ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(tmem_sfa), "r"(tmem_sfb) : "memory");
 }
+// Tile t in an order that keeps the tiles in flight near one another: eight row tiles high, so that 74 pairs of CTAs read about
+// 8 + 9 operand panels at a time instead of all the rows and one column (the panels then come from L2).
+__device__ __forceinline__ int2 tile_at(int t, int tiles_m, int tiles_n) {
+    const int band = t / (8 * tiles_n), first = band * 8, high = min(8, tiles_m - first), in = t - band * 8 * tiles_n;
+    return make_int2(first + in % high, in / high);
+}
 __device__ __forceinline__ float bias_at(const Gemm8Args& g, int64_t col) {
     float b[1];
     load_param<1>(g.bias, g.bias_dtype, col, b);
@@ -123,7 +129,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         uint32_t phase = 0;
         bool ok = true;
         for (int t = first_tile; t < total_tiles && ok; t += tile_step) {
-            const int tm = (t % g.tiles_m) * 2 + rank, tn = t / g.tiles_m;
+            const int2 tile = tile_at(t, g.tiles_m, g.tiles_n);
+            const int tm = tile.x * 2 + rank, tn = tile.y;
             for (int kt = 0; kt < g.k_tiles; ++kt) {
                 if (!mbar_wait_warp(&empty[stage], phase ^ 1, abort_flag)) { ok = false; break; }
                 if (elect_one()) {
@@ -217,7 +224,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             }
         };
         for (int t = first_tile; t < total_tiles; t += tile_step, ++local) {
-            const int tm = (t % g.tiles_m) * 2 + rank, tn = t / g.tiles_m;
+            const int2 tile = tile_at(t, g.tiles_m, g.tiles_n);
+            const int tm = tile.x * 2 + rank, tn = tile.y;
             const int acc = local & 1;
             if (!mbar_wait(&acc_full[acc], (local >> 1) & 1, abort_flag)) break;
             tc_fence_after();
@@ -560,4 +568,42 @@ extern "C" int nvfp4_fp8_gemm(const uint8_t* a, const uint8_t* a_scales, const u
     if (out_dtype == NVFP4_BF16) return launch_gemm8<__nv_bfloat16>(g, ma, mb, msa, msb, st);
     if (out_dtype == NVFP4_F16) return launch_gemm8<__half>(g, ma, mb, msa, msb, st);
     return launch_gemm8<float>(g, ma, mb, msa, msb, st);
+}
+
+extern "C" int64_t nvfp4_fp8_packing_bytes(int64_t rows, int64_t k) {
+    const int64_t kp = round128(k);
+    return rows * kp + round128(rows) / 128 * (kp / 128) * G8_SF;
+}
+
+static uint8_t* scales_of(const uint8_t* packing, int64_t rows, int64_t k) { return const_cast<uint8_t*>(packing) + rows * round128(k); }
+
+extern "C" int nvfp4_fp8_linear(const void* x, int x_dtype, int64_t m, int64_t k, int64_t x_pitch, const void* w, int w_dtype, int64_t n,
+                                int64_t w_pitch, const void* bias, int bias_dtype, void* y, uint8_t* work, uint8_t* x_t, uint8_t* w_t, int* status,
+                                nvfp4_stream_t stream) {
+    NVFP4_REQUIRE(x && w && y && work, NVFP4_ERR_ARG, "nvfp4_fp8_linear: null pointer");
+    NVFP4_REQUIRE(m > 0 && n > 0 && k > 0, NVFP4_ERR_ARG, "nvfp4_fp8_linear: sizes must be positive");
+    const bool packed = w_dtype == NVFP4_E4M3;
+    NVFP4_REQUIRE(!packed || !w_t, NVFP4_ERR_ARG, "nvfp4_fp8_linear: a packed weight has its transpose already");
+    uint8_t* wq = packed ? static_cast<uint8_t*>(const_cast<void*>(w)) : work + nvfp4_fp8_packing_bytes(m, k);
+    int rc = nvfp4_fp8_quantize(x, x_dtype, m, k, x_pitch, 0, work, scales_of(work, m, k), x_t, x_t ? scales_of(x_t, k, m) : nullptr, nullptr, stream);
+    if (!rc && !packed)
+        rc = nvfp4_fp8_quantize(w, w_dtype, n, k, w_pitch, 1, wq, scales_of(wq, n, k), w_t, w_t ? scales_of(w_t, k, n) : nullptr, nullptr, stream);
+    if (!rc)
+        rc = nvfp4_fp8_gemm(work, scales_of(work, m, k), wq, scales_of(wq, n, k), m, n, round128(k), bias, bias_dtype, y, x_dtype, n, status, stream);
+    return rc;
+}
+
+extern "C" int nvfp4_fp8_linear_bwd(const void* dy, int dtype, int64_t m, int64_t n, int64_t k, int64_t dy_pitch, const uint8_t* x_t,
+                                    const uint8_t* w_t, void* dx, void* dw, int dw_dtype, void* dbias, int dbias_dtype, uint8_t* work, int* status,
+                                    nvfp4_stream_t stream) {
+    NVFP4_REQUIRE(dy && work && (dx || dw || dbias) && (!dx || w_t) && (!dw || x_t), NVFP4_ERR_ARG, "nvfp4_fp8_linear_bwd: null pointer");
+    NVFP4_REQUIRE(m > 0 && n > 0 && k > 0, NVFP4_ERR_ARG, "nvfp4_fp8_linear_bwd: sizes must be positive");
+    uint8_t* g = dx ? work : nullptr;
+    uint8_t* g_t = dw || dbias ? work + (dx ? nvfp4_fp8_packing_bytes(m, n) : 0) : nullptr;
+    float* sums = dbias ? reinterpret_cast<float*>(g_t + nvfp4_fp8_packing_bytes(n, m)) : nullptr;
+    int rc = nvfp4_fp8_quantize(dy, dtype, m, n, dy_pitch, 0, g, g ? scales_of(g, m, n) : nullptr, g_t, g_t ? scales_of(g_t, n, m) : nullptr, sums, stream);
+    if (!rc && dx) rc = nvfp4_fp8_gemm(g, scales_of(g, m, n), w_t, scales_of(w_t, k, n), m, k, round128(n), nullptr, 0, dx, dtype, k, status, stream);
+    if (!rc && dw) rc = nvfp4_fp8_gemm(g_t, scales_of(g_t, n, m), x_t, scales_of(x_t, k, m), n, k, round128(m), nullptr, 0, dw, dw_dtype, k, status, stream);
+    if (!rc && dbias) rc = nvfp4_column_sums(sums, round128(m) / 128, n, dbias, dbias_dtype, stream);
+    return rc;
 }

@@ -54,6 +54,9 @@ _SIGNATURES = {
     "nvfp4_layer_norm_bwd": (I32, [P, I32, I64, P, I32, I64, P, P, P, I32, P, I64, I64, I64, P, P, P, P, P, P, P, P]),
     "nvfp4_fp8_quantize": (I32, [P, I32, I64, I64, I64, I32, P, P, P, P, P, P]),
     "nvfp4_fp8_gemm": (I32, [P, P, P, P, I64, I64, I64, P, I32, P, I32, I64, P, P]),
+    "nvfp4_fp8_packing_bytes": (I64, [I64, I64]),
+    "nvfp4_fp8_linear": (I32, [P, I32, I64, I64, I64, P, I32, I64, I64, P, I32, P, P, P, P, P, P]),
+    "nvfp4_fp8_linear_bwd": (I32, [P, I32, I64, I64, I64, I64, P, P, P, P, I32, P, I32, P, P, P]),
     "nvfp4_column_sums": (I32, [P, I64, I64, P, I32, P]),
     "nvfp4_rotary_axes": (I32, [P, I32, I32, I64, I64, I32, P, I32, P, I32, P, P, I32, I32, I32, P, P]),
     "nvfp4_gemm": (I32, [P, P, P, P, P, P, I64, I64, I64, P, I32, P, I32, I64, I64, I64, I32, P, P]),

@@ -25,76 +25,76 @@ def _ceil128(n):
     return (n + 127) // 128
 
 
+def _packing_bytes(rows, k):
+    """Codes [rows, k padded to 128] and their 512-byte scale blocks, as nvfp4_fp8_packing_bytes counts them."""
+    blocks = (k + 127) >> 7
+    return rows * blocks * 128 + ((rows + 127) >> 7) * blocks * 512
+
+
 @dataclass(frozen=True)
 class PackedFP8:
-    """A weight [rows, cols] laid out for the products: codes uint8 [rows, cols padded to 128], its scale blocks, and the same
-    of its transpose (None without it: then no gradient reaches the layer's input)."""
-    codes: torch.Tensor
-    scales: torch.Tensor
-    codes_t: Optional[torch.Tensor]
-    scales_t: Optional[torch.Tensor]
+    """A weight [rows, cols] laid out for the products: uint8 codes [rows, cols padded to 128] followed by their scale blocks,
+    and the same of its transpose (None without it: then no gradient reaches the layer's input)."""
+    packing: torch.Tensor
+    packing_t: Optional[torch.Tensor]
     shape: tuple
     dtype: torch.dtype
 
     @property
     def device(self):
-        return self.codes.device
+        return self.packing.device
 
     def dequantize(self):
         """FP32 [rows, cols]: the numbers the codes stand for."""
         rows, cols = self.shape
-        e = self.scales.view(_ceil128(rows), _ceil128(cols), 512)[:, :, 0].int() - 127
+        rb, cb = _ceil128(rows), _ceil128(cols)
+        codes = self.packing[:rows * cb * 128].view(rows, cb * 128)
+        e = self.packing[rows * cb * 128:].view(rb, cb, 512)[:, :, 0].int() - 127
         scale = ((e.long() + 1023) << 52).view(torch.float64).repeat_interleave(128, 0)[:rows].repeat_interleave(128, 1)      # 2^e
-        return (self.codes.view(torch.float8_e4m3fn).double() * scale)[:, :cols].float()
+        return (codes.view(torch.float8_e4m3fn).double() * scale)[:, :cols].float()
+
+
+def _bytes(n, device):
+    return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 def _quantize(x, *, row, col, square=False, column_sums=False):
-    """((codes, scales) or None, (codes_t, scales_t) or None, FP32 partial column sums or None) of x [rows, cols]."""
+    """(packing or None, transposed packing or None, FP32 partial column sums or None) of x [rows, cols]."""
     rows, cols = x.shape
-    rb, cb = _ceil128(rows), _ceil128(cols)
     dev = x.device
-    a, t, sums = (None, None), (None, None), None
-    if row:
-        a = (torch.empty((rows, cb * 128), dtype=torch.uint8, device=dev), torch.empty(rb * cb * 512, dtype=torch.uint8, device=dev))
-    if col:
-        t = (torch.empty((cols, rb * 128), dtype=torch.uint8, device=dev), torch.empty(cb * rb * 512, dtype=torch.uint8, device=dev))
-    if column_sums:
-        sums = torch.empty((rb, cols), dtype=torch.float32, device=dev)
+    a = _bytes(_packing_bytes(rows, cols), dev) if row else None
+    t = _bytes(_packing_bytes(cols, rows), dev) if col else None
+    sums = torch.empty((_ceil128(rows), cols), dtype=torch.float32, device=dev) if column_sums else None
+    at, tt = nat.ptr(a), nat.ptr(t)
     with nat.on(dev):
-        nat.check(nat.lib().nvfp4_fp8_quantize(x.data_ptr(), nat._CODES[x.dtype], rows, cols, pitch_of(x), square, nat.ptr(a[0]), nat.ptr(a[1]),
-                                               nat.ptr(t[0]), nat.ptr(t[1]), nat.ptr(sums), nat.raw_stream(dev)))
-    return (a if row else None), (t if col else None), sums
+        nat.check(nat.lib().nvfp4_fp8_quantize(x.data_ptr(), nat._CODES[x.dtype], rows, cols, pitch_of(x), square, at,
+                                               at and at + rows * _ceil128(cols) * 128, tt, tt and tt + cols * _ceil128(rows) * 128,
+                                               nat.ptr(sums), nat.raw_stream(dev)))
+    return a, t, sums
 
 
-def _gemm(a, b, k, dtype, bias=None, out=None):
-    """a, b: (codes, scales) of [M, k] and [N, k]."""
-    m, n = a[0].shape[0], b[0].shape[0]
-    dev = a[0].device
-    if out is None:
-        out = torch.empty((m, n), dtype=dtype, device=dev)
-    with nat.on(dev):
-        nat.check(nat.lib().nvfp4_fp8_gemm(a[0].data_ptr(), a[1].data_ptr(), b[0].data_ptr(), b[1].data_ptr(), m, n, _ceil128(k) * 128, nat.ptr(bias),
-                                           0 if bias is None else nat._CODES[bias.dtype], out.data_ptr(), nat._CODES[out.dtype], out.stride(0),
-                                           nat.status_word(dev).data_ptr(), nat.raw_stream(dev)))
-    return out
-
-
-def _column_sums(partial, dtype):
-    out = torch.empty(partial.shape[1], dtype=dtype, device=partial.device)
-    with nat.on(out.device):
-        nat.check(nat.lib().nvfp4_column_sums(partial.data_ptr(), partial.shape[0], partial.shape[1], out.data_ptr(), nat._CODES[dtype],
-                                              nat.raw_stream(out.device)))
-    return out
-
-
-def _inference(x, weight, bias, packed):
-    n, k = packed.shape if weight is None else weight.shape
+def _forward(x, weight, bias, packed, need_x, need_w):
+    """(y, transposed packing of x or None, that of the weight or None)."""
+    dev, codes = x.device, nat._CODES
+    if weight is None:
+        n, k = packed.shape
+        w, w_code, w_pitch, w_t, w_bytes = packed.packing, nat.E4M3, 0, None, 0
+    else:
+        n, k = weight.shape
+        w = rows_of(weight, k)
+        w_code, w_pitch, w_bytes = codes[w.dtype], pitch_of(w), _packing_bytes(n, k)
+        w_t = _bytes(_packing_bytes(k, n), dev) if need_x else None
     x2 = rows_of(x, k)
-    if not x2.shape[0]:
-        return torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
-    wq = (packed.codes, packed.scales) if weight is None else _quantize(rows_of(weight, k), row=True, col=False, square=True)[0]
-    y = _gemm(_quantize(x2, row=True, col=False)[0], wq, k, x.dtype, bias)
-    return y if x.ndim == 2 else y.view(*x.shape[:-1], n)
+    m = x2.shape[0]
+    y = torch.empty((m, n) if x.ndim == 2 else (*x.shape[:-1], n), dtype=x.dtype, device=dev)
+    x_t = _bytes(_packing_bytes(k, m), dev) if need_w else None
+    if m:
+        work = _bytes(_packing_bytes(m, k) + w_bytes, dev)
+        with nat.on(dev):
+            nat.check(nat.lib().nvfp4_fp8_linear(x2.data_ptr(), codes[x.dtype], m, k, pitch_of(x2), w.data_ptr(), w_code, n, w_pitch, nat.ptr(bias),
+                                                 0 if bias is None else codes[bias.dtype], y.data_ptr(), work.data_ptr(), nat.ptr(x_t), nat.ptr(w_t),
+                                                 nat.status_word(dev).data_ptr(), nat.raw_stream(dev)))
+    return y, x_t, (packed.packing_t if weight is None else w_t)
 
 
 class _Fp8Linear(torch.autograd.Function):
@@ -103,62 +103,58 @@ class _Fp8Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, packed):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        y, x_t, w_t = _forward(x, weight, bias, packed, need_x, need_w)
         n, k = packed.shape if weight is None else weight.shape
-        x2 = rows_of(x, k)
-        m = x2.shape[0]
-        ctx.dims, ctx.need, ctx.shape, ctx.dtype = (m, k, n), (need_x, need_w, need_b), x.shape, x.dtype
-        ctx.bias_dtype, ctx.weight_dtype = None if bias is None else bias.dtype, None if weight is None else weight.dtype
-        if m == 0:
-            ctx.save_for_backward(weight)
-            return torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
-        xq, xt, _ = _quantize(x2, row=True, col=need_w)
-        if weight is None:
-            wq, wt = (packed.codes, packed.scales), (packed.codes_t, packed.scales_t)
-        else:
-            wq, wt, _ = _quantize(rows_of(weight.detach(), k), row=True, col=need_x, square=True)
-        y = _gemm(xq, wq, k, x.dtype, bias)
-        ctx.save_for_backward(weight, *(wt if need_x else (None, None)), *(xt if need_w else (None, None)))
-        return y.view(*x.shape[:-1], n)
+        ctx.how = (x.numel() // k, n, k, need_x, need_w, None if not need_b else bias.dtype, x.shape, x.dtype)
+        ctx.save_for_backward(weight, w_t if need_x else None, x_t)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        m, k, n = ctx.dims
-        need_x, need_w, need_b = ctx.need
-        weight = ctx.saved_tensors[0]
-        if m == 0:
-            zero = lambda yes, shape, dtype: torch.zeros(shape, dtype=dtype, device=grad.device) if yes else None
-            return zero(need_x, ctx.shape, ctx.dtype), zero(need_w, (n, k), ctx.weight_dtype), zero(need_b, (n,), ctx.bias_dtype), None
-        _, wt_codes, wt_scales, xt_codes, xt_scales = ctx.saved_tensors
-        dx = dw = db = None
-        gq, gt, sums = _quantize(rows_of(grad, n), row=need_x, col=need_w or need_b, column_sums=need_b)
-        if need_x:
-            dx = _gemm(gq, (wt_codes, wt_scales), n, ctx.dtype).view(ctx.shape)
-        if need_w:
-            dw = _weight_gradient(weight, gt, (xt_codes, xt_scales), m)
-        if need_b:
-            db = _column_sums(sums, ctx.bias_dtype)
+        m, n, k, need_x, need_w, b_dtype, shape, dtype = ctx.how
+        weight, w_t, x_t = ctx.saved_tensors
+        dev = grad.device
+        dx = torch.empty(shape, dtype=dtype, device=dev) if need_x else None
+        db = None if b_dtype is None else torch.empty(n, dtype=b_dtype, device=dev)
+        if not m:
+            return dx, (torch.zeros(weight.shape, dtype=weight.dtype, device=dev) if need_w else None), (None if db is None else db.zero_()), None
+        dw, taken = _weight_gradient_into(weight) if need_w else (None, None)
+        columns = need_w or db is not None
+        work = _bytes((_packing_bytes(m, n) if need_x else 0) + (_packing_bytes(n, m) + 4 * n * _ceil128(m) if columns else 0), dev)
+        g = rows_of(grad, n)
+        codes = nat._CODES
+        with nat.on(dev):
+            nat.check(nat.lib().nvfp4_fp8_linear_bwd(g.data_ptr(), codes[g.dtype], m, n, k, pitch_of(g), nat.ptr(x_t), nat.ptr(w_t), nat.ptr(dx), nat.ptr(dw),
+                                                     0 if dw is None else codes[dw.dtype], nat.ptr(db), 0 if db is None else codes[b_dtype],
+                                                     work.data_ptr(), nat.status_word(dev).data_ptr(), nat.raw_stream(dev)))
+        if taken is not None:
+            taken(dw)
+            dw = None
         return dx, dw, db, None
 
 
-def _weight_gradient(weight, gt, xt, tokens):
-    """dW, or None where an optimizer that collects gradients itself (backward_step, captured steps) has taken it."""
+def _weight_gradient_into(weight):
+    """(tensor that receives dW, None), or with a function that hands it on where an optimizer collects gradients itself
+    (backward_step, captured steps) instead of autograd."""
+    new = lambda dtype: torch.empty(weight.shape, dtype=dtype, device=weight.device)
     sink = getattr(weight, "_v4_pending", None)
     if sink is None or weight.numel() < 4096:          # smaller weights have FP32 moments and take an ordinary gradient
-        return _gemm(gt, xt, tokens, weight.dtype)
+        return new(weight.dtype), None
     reducer = getattr(weight, "_dp_reducer", None)
     if reducer is not None:
         if weight in sink:
             raise RuntimeError("An 8-bit layer may be applied only once per step under data parallel")
         slot = reducer.slot(weight)
-        _gemm(gt, xt, tokens, slot.dtype, out=slot.view(weight.shape))
-        sink[weight] = (slot, None, None)
-        reducer.ready(weight)
-    elif weight in sink:                                # a layer applied twice: the sum stays in FP32
-        sink[weight] = (_gemm(gt, xt, tokens, torch.float32).add_(sink[weight][0]), None, None)
-    else:
-        sink[weight] = (_gemm(gt, xt, tokens, torch.float32 if weight.dtype == torch.float32 else torch.bfloat16), None, None)
-    return None
+
+        def reduce(_):
+            sink[weight] = (slot, None, None)
+            reducer.ready(weight)
+        return slot.view(weight.shape), reduce
+
+    def keep(dw):                                       # a layer applied twice: the sum stays in FP32
+        sink[weight] = (dw.add_(sink[weight][0]) if weight in sink else dw, None, None)
+    return new(torch.float32 if weight in sink or weight.dtype == torch.float32 else torch.bfloat16), keep
 
 
 def fp8_pack(weight, *, transpose=True):
@@ -168,9 +164,8 @@ def fp8_pack(weight, *, transpose=True):
     if weight.ndim != 2 or 0 in weight.shape or max(weight.shape) >= _MAX:
         raise ValueError("weight must be [out_features, in_features], not empty")
     _check_device(weight)
-    w = rows_of(weight.detach(), weight.shape[1])
-    q, t, _ = _quantize(w, row=True, col=transpose, square=True)
-    return PackedFP8(*q, *(t if transpose else (None, None)), tuple(weight.shape), weight.dtype)
+    q, t, _ = _quantize(rows_of(weight.detach(), weight.shape[1]), row=True, col=transpose, square=True)
+    return PackedFP8(q, t, tuple(weight.shape), weight.dtype)
 
 
 def fp8_linear(x, weight, bias=None):
@@ -192,13 +187,13 @@ def fp8_linear(x, weight, bias=None):
         _check_tensor("bias", bias)
         if bias.shape != (weight.shape[0],) or bias.device != x.device or not bias.is_contiguous():
             raise ValueError(f"bias must be a contiguous vector of {weight.shape[0]} features on the input's device")
-    if packed is not None and packed.codes_t is None and x.requires_grad and torch.is_grad_enabled():
+    if packed is not None and packed.packing_t is None and x.requires_grad and torch.is_grad_enabled():
         raise ValueError("This weight was packed without its transpose: no gradient can reach x")
     _check_device(x)
     if packed is not None:
         weight = None
     if not (torch.is_grad_enabled() and (x.requires_grad or any(t is not None and t.requires_grad for t in (weight, bias)))):
-        return _inference(x, weight, bias, packed)
+        return _forward(x, weight, bias, packed, False, False)[0]
     return _Fp8Linear.apply(x, weight, bias, packed)
 
 

@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from functools import lru_cache
 
 import torch
@@ -192,27 +193,34 @@ class LayerNorm(nn.LayerNorm):
 # ---- rotary positions over several axes -----------------------------------------------------------------------------------
 _POSITION_KINDS = {torch.int64: 0, torch.int32: 1, torch.float32: 2, torch.float64: 3}
 MAX_PAIRS = 256
-_Strides = C.c_int64 * 3
 
 
-class _Tensor(C.Structure):
-    _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("x_stride", C.c_int64 * 3), ("out_stride", C.c_int64 * 3), ("heads", C.c_int32),
-                ("turn", C.c_int32)]
+_JOB = struct.Struct("=QQqqqqqqii")       # nvfp4_rotary_tensor
+_STRIDES = struct.Struct("=qqq")
 
 
 @lru_cache(maxsize=256)
-def _plan(sections, theta, frequencies):
-    """Host arrays for the kernel: frequency / (2 pi) and axis of every pair."""
+def _plan(sections, dim, theta, layout, frequencies):
+    """Checked once per set of arguments: (host arrays of frequency / (2 pi) and axis of every pair, pairs), axes, interleaved."""
+    if not sections or any(type(n) is not int or n < 1 for n in sections):
+        raise ValueError("sections must be positive integers: the pairs of a head that each position axis turns")
     pairs = sum(sections)
+    if 2 * pairs > dim or pairs > MAX_PAIRS:
+        raise ValueError(f"sections hold {pairs} pairs; a head of {dim} features has room for {min(dim // 2, MAX_PAIRS)}")
+    if layout not in ("half", "interleaved"):
+        raise ValueError("layout must be 'half' or 'interleaved'")
+    if frequencies not in ("shared", "axis"):
+        raise ValueError("frequencies must be 'shared' or 'axis'")
+    if not (math.isfinite(theta) and theta > 0):
+        raise ValueError("theta must be positive and finite")
     turns, axis = (C.c_double * pairs)(), (C.c_uint8 * pairs)()
     j = 0
     for a, n in enumerate(sections):
         for i in range(n):
-            exponent = i / n if frequencies == "axis" else j / pairs
-            turns[j] = theta ** -exponent / (2 * math.pi)
+            turns[j] = theta ** -(i / n if frequencies == "axis" else j / pairs) / (2 * math.pi)
             axis[j] = a
             j += 1
-    return turns, axis, pairs
+    return (turns, axis, pairs), len(sections), layout == "interleaved"
 
 
 def _launch_rotary(jobs, positions, plan, axes, interleaved, inverse, amax):
@@ -220,12 +228,12 @@ def _launch_rotary(jobs, positions, plan, axes, interleaved, inverse, amax):
     x0 = jobs[0][0]
     batch, seq, _, dim = x0.shape
     turns, axis, pairs = plan
-    tensors = (_Tensor * len(jobs))(*[(x.data_ptr(), out.data_ptr(), x.stride()[:3], out.stride()[:3], x.shape[2], turn) for x, out, turn in jobs])
+    tensors = b"".join([_JOB.pack(x.data_ptr(), out.data_ptr(), *x.stride()[:3], *out.stride()[:3], x.shape[2], turn) for x, out, turn in jobs])
     ps = positions.stride() if positions.ndim == 3 else (0, *positions.stride())
     dev = x0.device
     with nat.on(dev):
         nat.check(nat.lib().nvfp4_rotary_axes(tensors, len(jobs), nat._CODES[x0.dtype], batch, seq, dim, positions.data_ptr(),
-                                              _POSITION_KINDS[positions.dtype], _Strides(*ps), axes, turns, axis, pairs, interleaved, inverse,
+                                              _POSITION_KINDS[positions.dtype], _STRIDES.pack(*ps), axes, turns, axis, pairs, interleaved, inverse,
                                               nat.ptr(amax), nat.raw_stream(dev)))
 
 
@@ -294,23 +302,13 @@ class _RotaryFused(torch.autograd.Function):
 
 
 def _check_rotary(x, batch, seq, dim, positions, sections, theta, layout, frequencies):
-    sections = tuple(sections)
-    if not sections or any(type(n) is not int or n < 1 for n in sections):
-        raise ValueError("sections must be positive integers: the pairs of a head that each position axis turns")
-    if 2 * sum(sections) > dim or sum(sections) > MAX_PAIRS:
-        raise ValueError(f"sections hold {sum(sections)} pairs; a head of {dim} features has room for {min(dim // 2, MAX_PAIRS)}")
-    if layout not in ("half", "interleaved"):
-        raise ValueError("layout must be 'half' or 'interleaved'")
-    if frequencies not in ("shared", "axis"):
-        raise ValueError("frequencies must be 'shared' or 'axis'")
-    theta = float(theta)
-    if not (math.isfinite(theta) and theta > 0):
-        raise ValueError("theta must be positive and finite")
-    _check_tensor("positions", positions, tuple(_POSITION_KINDS))
-    if positions.device != x.device or positions.shape not in ((seq, len(sections)), (batch, seq, len(sections))):
-        raise ValueError(f"positions must be [{seq}, {len(sections)}] or [{batch}, {seq}, {len(sections)}] on the input's device")
+    how = _plan(tuple(sections), dim, float(theta), layout, frequencies)
+    _check_tensor("positions", positions, _POSITION_KINDS)
+    shape = positions.shape
+    if positions.device != x.device or shape[-2:] != (seq, how[1]) or not (len(shape) == 2 or (len(shape) == 3 and shape[0] == batch)):
+        raise ValueError(f"positions must be [{seq}, {how[1]}] or [{batch}, {seq}, {how[1]}] on the input's device")
     _check_device(x)
-    return _plan(sections, theta, frequencies), len(sections), layout == "interleaved"
+    return how
 
 
 def rotary_axes(q, k, positions, sections, *, theta=10000.0, layout="half", frequencies="shared"):

@@ -73,7 +73,7 @@ def test_rotary_refusals(error, call):
 
 def test_entry_points_refuse_before_any_launch():
     from nvfp4_training import _native
-    from nvfp4_training.operators import _Tensor
+    from nvfp4_training.operators import _JOB
     lib = _native.lib()
     buf = C.create_string_buffer(4096)
 
@@ -87,12 +87,11 @@ def test_entry_points_refuse_before_any_launch():
     assert bwd(dw=buf) == 1 and bwd(dd=buf) == 3 and bwd(xd=2, hd=1) == 3
     assert lib.nvfp4_layer_norm_bwd_partials(1, 8) == 1 and lib.nvfp4_layer_norm_bwd_partials(10 ** 9, 8) <= 1024
 
-    tensors = (_Tensor * 1)()
     turns, axis, strides = (C.c_double * 300)(), (C.c_uint8 * 300)(), (C.c_int64 * 3)()
 
     def rotary(count=1, dtype=1, dim=16, kind=0, axes=1, pairs=8, heads=2, address=None):
-        tensors[0].x = tensors[0].out = C.addressof(buf) if address is None else address
-        tensors[0].heads, tensors[0].turn = heads, 1
+        at = C.addressof(buf) if address is None else address
+        tensors = _JOB.pack(at, at, 0, 0, 0, 0, 0, 0, heads, 1) * 4
         return lib.nvfp4_rotary_axes(tensors, count, dtype, 1, 4, dim, buf, kind, strides, axes, turns, axis, pairs, 0, 0, None, None)
     assert rotary(count=0) == 1 and rotary(count=4) == 1 and rotary(dtype=3) == 3 and rotary(kind=4) == 3 and rotary(pairs=9) == 1
     assert rotary(dim=600, pairs=257) == 1 and rotary(heads=0) == 1 and rotary(address=0) == 1
@@ -128,7 +127,7 @@ def test_fp8_refusals(error, call):
 
 
 def test_packed_weight_without_its_transpose_refuses_input_gradients():
-    packed = nv.PackedFP8(torch.zeros(6, 128, dtype=torch.uint8), torch.full((512,), 127, dtype=torch.uint8), None, None, (6, 16), BF16)
+    packed = nv.PackedFP8(torch.cat([torch.zeros(6 * 128, dtype=torch.uint8), torch.full((512,), 127, dtype=torch.uint8)]), None, (6, 16), BF16)
     assert packed.dequantize().shape == (6, 16)
     with pytest.raises(ValueError, match="transpose"):
         nv.fp8_linear(x(2, 16).requires_grad_(True), packed)
@@ -153,6 +152,12 @@ def test_fp8_entry_points_refuse_before_any_launch():
     assert gemm(a=None) == 1 and gemm(out=None) == 1 and gemm(m=0) == 1 and gemm(n=0) == 1 and gemm(k=64) == 1 and gemm(ldo=7) == 1
     assert gemm(k=0) == 1 and gemm(m=1 << 30) == 1 and gemm(m=1 << 29, n=1 << 29, ldo=1 << 29) == 1
     assert gemm(od=3) == 3 and gemm(bias=at, bd=4) == 3 and gemm(a=at + 8) == 2 and gemm(out=at + 1) == 2
+    from nvfp4_training.fp8 import _packing_bytes
+    assert all(lib.nvfp4_fp8_packing_bytes(r, k) == _packing_bytes(r, k) for r in (1, 127, 128, 129) for k in (1, 128, 300))
+    linear = lambda x=at, work=at, m=4, wd=1, w_t=None: lib.nvfp4_fp8_linear(x, 1, m, 128, 128, at, wd, 8, 128, None, 0, at, work, None, w_t, None, None)
+    assert linear(x=None) == 1 and linear(work=None) == 1 and linear(m=0) == 1 and linear(wd=3, w_t=at) == 1
+    back = lambda dx=None, dw=None, x_t=None, w_t=None, m=4: lib.nvfp4_fp8_linear_bwd(at, 1, m, 8, 128, 8, x_t, w_t, dx, dw, 1, None, 0, at, None, None)
+    assert back() == 1 and back(dx=at) == 1 and back(dw=at) == 1 and back(dx=at, w_t=at, m=0) == 1
     assert lib.nvfp4_column_sums(at, 0, 8, at, 0, None) == 1 and lib.nvfp4_column_sums(at, 1, 8, at, 3, None) == 3
 
 

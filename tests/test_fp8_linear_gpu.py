@@ -30,9 +30,10 @@ def quantised(x, block_rows, block_cols):
     return q.reshape(t.shape[0] * block_rows, -1)[:rows, :cols], e[:, 0, :, 0]
 
 
-def codes_to_values(codes, scales, rows, cols):
-    """What codes [rows, cols_p] and their swizzled scale blocks stand for, and the exponent of every (row, block)."""
+def codes_to_values(packing, rows, cols):
+    """What codes [rows, cols_p] and the swizzled scale blocks behind them stand for, and the exponent of every (row, block)."""
     rb, cb = -(-rows // 128), -(-cols // 128)
+    codes, scales = packing[:rows * cb * 128].view(rows, cb * 128), packing[rows * cb * 128:]
     words = scales.view(rb, cb, 32, 4, 4)                                  # row % 32, row / 32, four copies
     assert bool((words == words[..., :1]).all())
     e = words[..., 0].permute(0, 3, 2, 1).reshape(rb * 128, cb).int() - 127
@@ -59,17 +60,17 @@ def test_codes_and_scales(rows, cols, dtype, square):
     q, t, sums = _quantize(x, row=True, col=True, square=square, column_sums=True)
     shape = (128, 128) if square else (1, 128)
     want, e = quantised(x, *shape)
-    got, ge = codes_to_values(*q, rows, cols)
+    got, ge = codes_to_values(q, rows, cols)
     assert torch.equal(got[:, :cols], want) and not got[:, cols:].any()
     assert torch.equal(ge[:rows], e.repeat_interleave(128, 0)[:rows] if square else e)
     want, e = quantised(x.t(), *shape)
-    got, ge = codes_to_values(*t, cols, rows)
+    got, ge = codes_to_values(t, cols, rows)
     assert torch.equal(got[:, :rows], want) and not got[:, rows:].any()
     assert torch.equal(ge[:cols], e.repeat_interleave(128, 0)[:cols] if square else e)
     block_sums = torch.nn.functional.pad(x.double(), (0, 0, 0, -rows % 128)).view(-1, 128, cols).sum(1)
     assert bool(((sums.double() - block_sums).abs() <= 2.0 ** -20 * x.double().abs().sum(0)).all())
     only, none, _ = _quantize(x, row=True, col=False, square=square)
-    assert none is None and torch.equal(only[0], q[0]) and torch.equal(only[1], q[1])
+    assert none is None and torch.equal(only, q)
 
 
 def test_range_of_the_scale():
@@ -81,8 +82,8 @@ def test_range_of_the_scale():
     x[2, 0], x[2, 1] = 2.0 ** -133, -(2.0 ** -133)
     x[3, 5], x[4, 6], x[5, 7] = float("inf"), float("-inf"), float("nan")
     x[3:6, 128:] = 1.5
-    (codes, scales), _, _ = _quantize(x, row=True, col=False)
-    got, e = codes_to_values(codes, scales, 8, 256)
+    packing, _, _ = _quantize(x, row=True, col=False)
+    got, e = codes_to_values(packing, 8, 256)
     want, we = quantised(x[:3], 1, 128)
     assert torch.equal(got[:3], want) and torch.equal(e[:3], we)
     assert got[3:6, :128].isnan().all() and torch.equal(got[3:6, 128:], x[3:6, 128:].double()) and not got[6:].any()
