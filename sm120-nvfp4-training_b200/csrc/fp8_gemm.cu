@@ -8,9 +8,10 @@
 //   fp8_gemm_kernel        persistent clusters of two CTAs on 256 x 256 tiles (cta_group::2, M256 x N256 x K32 instructions), for
 //                          problems that fill the GPU with such tiles.  Tensor issue and the shared-memory bandwidth under
 //                          it are the bound.
-//   fp8_gemm_split_kernel  one 128 x 128 tile per cluster of 1 to 8 CTAs, each with a share of the contraction; the FP32
-//                          partial tiles are added through distributed shared memory in rank order.  For few rows (the weight
-//                          is read once, HBM or latency is the bound) and for problems of few tiles.
+//   fp8_gemm_split_kernel  one tile of up to 128 rows of A and 128 of B per cluster of 1 to 8 CTAs, each with a share of the
+//                          contraction; the FP32 partial tiles are added through distributed shared memory in rank order.  B's
+//                          rows are the 128 of the instruction and A's its columns, so that few rows of A cost what they are
+//                          (sixteens).  For few rows (the weight is read once, HBM or latency is the bound) and few tiles.
 // The host picks by the estimated number of cycles of each (split_for below).
 // Operands are unpadded in M and N: tile loads beyond the tensor arrive as zeros, stores are cropped.
 // Every wait is bounded as in the NVFP4 GEMM: on expiry the status word is raised, all roles leave, and the kernel returns.
@@ -31,7 +32,7 @@ struct Gemm8Args {
     void* out;
     int* status;
     int64_t ldo;
-    int bias_dtype, M, N, k_tiles, tiles_m, tiles_n, tma_store;
+    int bias_dtype, M, N, k_tiles, tiles_m, tiles_n, tma_store, a_rows;      // a_rows: rows of A per tile of the split kernel
 };
 
 __device__ __forceinline__ uint32_t instr_desc8(int n, int m) {    // e4m3 x e4m3, UE8M0 scales, K-major A and B
@@ -79,9 +80,9 @@ constexpr int STAGE_BYTES = OPERANDS + SCALES;
 // Tensor memory: two accumulators of 256 columns that share 32 ([0, 256) and [224, 480)), so that two scale buffers of
 // 4 + 8 columns fit behind them.  The epilogue reads the shared columns first, and only that read gates the next tile.
 constexpr int ACC_STRIDE = 224, SF_BASE = 480, SF_COLS = 12, TMEM_COLS = 512;
-constexpr int SLAB = 1024;                           // 32 rows x 32 bytes per epilogue warp
+constexpr int SLAB = 1024;                           // 32 rows x 32 bytes, two per epilogue warp
 constexpr int BARS = 2 * STAGES + 4;
-constexpr int SMEM = STAGES * STAGE_BYTES + EPI_WARPS * SLAB + 1024 + 256;
+constexpr int SMEM = STAGES * STAGE_BYTES + EPI_WARPS * 2 * SLAB + 1024 + 256;
 static_assert(SF_BASE + 2 * SF_COLS <= TMEM_COLS && BARS * 8 + 16 <= 256 && SMEM <= 232448, "budgets");
 }  // namespace pair8
 
@@ -93,7 +94,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* epi_smem = smem + STAGES * OPERANDS;
-    uint8_t* sf_smem = epi_smem + EPI_WARPS * SLAB;
+    uint8_t* sf_smem = epi_smem + EPI_WARPS * 2 * SLAB;
     uint64_t* full = reinterpret_cast<uint64_t*>(sf_smem + STAGES * SCALES);
     uint64_t* empty = full + STAGES;
     uint64_t* acc_full = empty + STAGES;
@@ -199,12 +200,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         // ---- epilogue: two warps per TMEM sub-partition, eight 16-column units of the tile each ----
         constexpr int ESZ = sizeof(TO);
         const int sub = warp & 3, half = (warp - FIRST_EPI_WARP) >> 2;
-        uint8_t* slab = epi_smem + (warp - FIRST_EPI_WARP) * SLAB;
-        int local = 0;
-        // 32 rows x 32 bytes, two uint4 per lane: through the staging slab and a TMA store (which crops), or directly
+        uint8_t* slabs = epi_smem + (warp - FIRST_EPI_WARP) * 2 * SLAB;
+        int local = 0, turn = 0;
+        // 32 rows x 32 bytes, two uint4 per lane: through one of two staging slabs and a TMA store (which crops), or directly.
+        // (Each lane storing its row's 32 bytes itself was slower wherever tiles end together: 4304 x 1152 x 1000 17.5 against 13.8 us.)
         auto emit = [&](const uint4& q0, const uint4& q1, int64_t row, int64_t col0, int tile_row0) {
             if (g.tma_store) {
-                if (lane == 0) bulk_wait_read<0>();
+                uint8_t* slab = slabs + (turn ^= SLAB);
+                if (lane == 0) bulk_wait_read<1>();      // the store before the last has read this slab
                 __syncwarp();
                 const int sw = (lane >> 2) & 1;
                 *reinterpret_cast<uint4*>(slab + lane * 32 + (sw << 4)) = q0;
@@ -294,13 +297,20 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 // one 128 x 128 tile per cluster, the contraction split over its CTAs
 // ====================================================================================================================
 namespace split8 {
-constexpr int THREADS = 192, STAGES = 6;
-constexpr int OPERANDS = 2 * G8_OPERAND, SCALES = 2 * G8_SF, STAGE_BYTES = OPERANDS + SCALES;
+constexpr int THREADS = 192, MAX_STAGES = 12;
+constexpr int SCALES = 2 * G8_SF;
 constexpr int SF_BASE = 128, SF_COLS = 8, TMEM_COLS = 256;
 constexpr int PITCH = 132;                           // floats per row of the partial tile: lanes of a quarter warp hit different banks
-constexpr int BARS = 2 * STAGES + 1;
-constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256;
-static_assert(128 * PITCH * 4 <= STAGES * OPERANDS && BARS * 8 + 16 <= 256 && SMEM <= 232448, "budgets");
+constexpr int BARS = 2 * MAX_STAGES + 1;
+constexpr int FIXED = 1024 + 256;
+constexpr int SMEM = 6 * (2 * G8_OPERAND + SCALES) + FIXED;
+// Bytes in flight are what a few rows need (their k-tiles come from HBM at its latency): fewer rows of A, more stages.
+__host__ __device__ constexpr int operands(int a_rows) { return (a_rows + 128) * 128; }
+__host__ __device__ constexpr int stages(int a_rows) {
+    const int n = (SMEM - FIXED) / (operands(a_rows) + SCALES);
+    return n < MAX_STAGES ? n : MAX_STAGES;
+}
+static_assert(128 * PITCH * 4 <= stages(128) * operands(128) && 16 * PITCH * 4 <= stages(16) * operands(16) && BARS * 8 + 16 <= 256 && SMEM <= 232448, "budgets");
 }  // namespace split8
 
 __device__ __forceinline__ float4 cluster_load4(uint32_t addr, int rank) {     // 16 bytes at this shared-memory offset of CTA `rank`
@@ -318,10 +328,11 @@ fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     using namespace split8;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* sf_smem = smem + STAGES * OPERANDS;
-    uint64_t* full = reinterpret_cast<uint64_t*>(sf_smem + STAGES * SCALES);
-    uint64_t* empty = full + STAGES;
-    uint64_t* acc_full = empty + STAGES;
+    const int depth = stages(g.a_rows), stage_operands = operands(g.a_rows);
+    uint8_t* sf_smem = smem + depth * stage_operands;
+    uint64_t* full = reinterpret_cast<uint64_t*>(sf_smem + depth * SCALES);
+    uint64_t* empty = full + depth;
+    uint64_t* acc_full = empty + depth;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -331,7 +342,7 @@ fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     const int tm = tile % g.tiles_m, tn = tile / g.tiles_m;
     const int k0 = static_cast<int>(static_cast<int64_t>(g.k_tiles) * rank / splits), k1 = static_cast<int>(static_cast<int64_t>(g.k_tiles) * (rank + 1) / splits);
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < depth; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         mbar_init(acc_full, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -346,66 +357,67 @@ fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     const uint32_t tmem_base = *tmem_slot;
 
     if (warp == 0) {
+        // a stage holds 128 rows of B, then a_rows of A
         bool ok = true;
-        int kt = k0;
-        for (int i = 0; kt < k1; ++kt, ++i) {
-            const int stage = i % STAGES;
-            if (!mbar_wait_warp(&empty[stage], ((i / STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
+        int kt = k0, stage = 0, filled = 0;
+        uint32_t phase = 1;
+        for (; kt < k1; ++kt) {
+            if (!mbar_wait_warp(&empty[stage], phase, abort_flag)) { ok = false; break; }
             if (elect_one()) {
-                uint8_t* st = smem + stage * OPERANDS;
+                uint8_t* st = smem + stage * stage_operands;
                 uint8_t* sf = sf_smem + stage * SCALES;
-                mbar_expect_tx(&full[stage], STAGE_BYTES);
-                tma_load_2d(st + G8_OPERAND, &map_b, kt * G8_BK, tn * 128, &full[stage]);
-                tma_load_2d(st, &map_a, kt * G8_BK, tm * 128, &full[stage]);
+                mbar_expect_tx(&full[stage], stage_operands + SCALES);
+                tma_load_2d(st, &map_b, kt * G8_BK, tn * 128, &full[stage]);
+                tma_load_2d(st + G8_OPERAND, &map_a, kt * G8_BK, tm * 128, &full[stage]);
                 tma_load_2d(sf, &map_sfa, 0, tm * g.k_tiles + kt, &full[stage]);
                 tma_load_2d(sf + G8_SF, &map_sfb, 0, tn * g.k_tiles + kt, &full[stage]);
             }
             __syncwarp();
+            filled = min(filled + 1, depth);
+            if (++stage == depth) { stage = 0; phase ^= 1; }
         }
         if (!ok && lane == 0) {      // a bounded chance for the loads in flight to land
-            for (int i = max(0, kt - k0 - STAGES); i < kt - k0; ++i) {
+            for (int i = 0; i < filled; ++i) {
+                if (--stage < 0) { stage = depth - 1; phase ^= 1; }
                 const long long t0 = clock64();
-                while (!mbar_try(&full[i % STAGES], (i / STAGES) & 1) && clock64() - t0 < WAIT_CYCLES / 8) {}
+                while (!mbar_try(&full[stage], phase ^ 1) && clock64() - t0 < WAIT_CYCLES / 8) {}
             }
         }
     } else if (warp == 1) {
-        const uint32_t idesc = instr_desc8(128, 128);
+        const uint32_t idesc = instr_desc8(g.a_rows, 128);      // B's rows are the instruction's 128, A's its columns
         bool ok = true;
+        int stage = 0;
+        uint32_t phase = 0;
         for (int i = 0; i < k1 - k0; ++i) {
-            const int stage = i % STAGES;
-            if (!mbar_wait_warp(&full[stage], (i / STAGES) & 1, abort_flag)) { ok = false; break; }
+            if (!mbar_wait_warp(&full[stage], phase, abort_flag)) { ok = false; break; }
             tc_fence_after();
             if (elect_one()) {
-                const uint32_t sa = smem_u32(smem + stage * OPERANDS), sb = sa + G8_OPERAND, sf = smem_u32(sf_smem + stage * SCALES);
+                const uint32_t sb = smem_u32(smem + stage * stage_operands), sa = sb + G8_OPERAND, sf = smem_u32(sf_smem + stage * SCALES);
                 const uint32_t tsfa = tmem_base + SF_BASE + (i & 1) * SF_COLS, tsfb = tsfa + 4;
-                tc_cp_sf(tsfa, scale_desc(sf));
-                tc_cp_sf(tsfb, scale_desc(sf + G8_SF));
+                tc_cp_sf(tsfa, scale_desc(sf + G8_SF));
+                tc_cp_sf(tsfb, scale_desc(sf));
 #pragma unroll
                 for (int kb = 0; kb < 4; ++kb)
-                    mma8<false>(tmem_base, operand_desc(sa + kb * 32), operand_desc(sb + kb * 32), idesc, (i | kb) ? 1u : 0u, tsfa, tsfb);
+                    mma8<false>(tmem_base, operand_desc(sb + kb * 32), operand_desc(sa + kb * 32), idesc, (i | kb) ? 1u : 0u, tsfa, tsfb);
                 tc_commit(&empty[stage]);
             }
             __syncwarp();
+            if (++stage == depth) { stage = 0; phase ^= 1; }
         }
         if (ok && elect_one()) tc_commit(acc_full);
         __syncwarp();
     } else if (mbar_wait_warp(acc_full, 0, abort_flag)) {
-        // every MMA has read its operands: their shared memory takes the FP32 partial tile, one row per lane
+        // every MMA has read its operands: their shared memory takes the FP32 partial tile [rows of A][128]; a lane holds a
+        // column of it
         tc_fence_after();
-        const int row = (warp & 3) * 32 + lane;
         const uint32_t taddr = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-        float* mine = reinterpret_cast<float*>(smem) + row * PITCH;
-        const bool live = tm * 128 + row < g.M;
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
+        float* mine = reinterpret_cast<float*>(smem) + (warp & 3) * 32 + lane;
+        for (int u = 0; u < g.a_rows; u += 16) {
             uint32_t r[16];
-            tc_ld16(taddr + u * 16, r);
+            tc_ld16(taddr + u, r);
             tc_wait_ld();
-            if (live) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    *reinterpret_cast<uint4*>(mine + u * 16 + j * 4) = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-            }
+            for (int j = 0; j < 16; ++j) mine[(u + j) * PITCH] = __uint_as_float(r[j]);
         }
     }
     tc_fence_before();
@@ -469,44 +481,71 @@ static bool map_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base,
     return fn(map, type, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-static bool operand_map(CUtensorMap* map, const uint8_t* base, int64_t rows, int64_t k) {
-    return map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, k, rows, k, G8_BK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+static bool operand_map(CUtensorMap* map, const uint8_t* base, int64_t rows, int64_t k, int box_rows) {
+    return map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, k, rows, k, G8_BK, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 static bool scale_map(CUtensorMap* map, const uint8_t* base, int64_t rows, int64_t k) {      // one 512-byte block per row
     return map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, G8_SF / 4, (rows + 127) / 128 * (k / 128), G8_SF, G8_SF / 4, 1, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-// 0: paired CTAs on 256 x 256 tiles; else the number of CTAs that share a 128 x 128 tile's contraction.  Estimated cycles: a
-// stage of the paired kernel takes 512 (its four instructions at the tensor cores' rate), one of the split kernel about 300
-// (256 of tensor time, plus its operands' shared-memory reads, which N = 128 instructions do not hide); a tile costs about
-// 1500 more for filling the pipeline and draining it, joining partial tiles another 1500.
-static int split_for(const Gemm8Args& g, int sms) {
+// 0: paired CTAs on 256 x 256 tiles; else the number of CTAs that share a tile's contraction.  The smallest of the times that a
+// fit to measurements gives, in ns (16 shapes from 1 x 4096 x 128 to 16384 x 4096 x 14336; within 20 %, and the fastest way
+// picked for each): paired, 8 us and 360 ns per k-tile of every wave (its tensor time at 1.4 GHz); split, 1.5 us and per wave
+// a start and end of 2 to 4.5 us (3.2 to 6.5 in a cluster) and 240 to 390 ns per k-tile by the rows of A, which is the
+// operands' way from L2 rather than their products.  For example 1 x 4096 x 4096: paired 17.0 us, one CTA a tile 10.7, two 8.8,
+// four 8.0, eight (three waves of clusters) 17.3; 1000 x 1152 x 4304: 18.0, 15.8, 13.6, 31.1; 2048 x 2048 x 2048: 13.8, 22.2.
+struct Slots { int clusters[4]; int pairs; };        // tiles in flight: split clusters of 1, 2, 4, 8 CTAs; paired CTAs
+static int split_for(const Gemm8Args& g, const Slots& slots) {
     auto waves = [](int64_t work, int64_t slots) { return (work + slots - 1) / slots; };
-    int64_t best = waves(static_cast<int64_t>((g.M + 255) / 256) * ((g.N + 255) / 256), sms / 2) * (g.k_tiles * 512LL + 1500);
+    const int64_t pair_waves = waves(static_cast<int64_t>((g.M + 255) / 256) * ((g.N + 255) / 256), slots.pairs);
+    int64_t best = 8000 + pair_waves * g.k_tiles * 360 + (pair_waves - 1) * 600;
     int pick = 0;
     const int64_t tiles = static_cast<int64_t>((g.M + 127) / 128) * ((g.N + 127) / 128);
-    for (int s = 1; s <= 8 && s <= g.k_tiles; s *= 2) {
-        const int64_t cost = waves(tiles * s, sms) * (waves(g.k_tiles, s) * 300LL + 1500) + (s > 1 ? 1500 : 0);
+    for (int s = 1, i = 0; s <= 8 && s <= g.k_tiles && slots.clusters[i]; s *= 2, ++i) {
+        const int64_t ends = s > 1 ? 3200 + 26 * g.a_rows : 2000 + 20 * g.a_rows;
+        const int64_t cost = 1500 + waves(tiles, slots.clusters[i]) * (ends + waves(g.k_tiles, s) * (240 + g.a_rows * 6 / 5));
         if (cost < best) { best = cost; pick = s; }
     }
     return pick;
 }
 
 template <typename TO>
-static int launch_gemm8(Gemm8Args& g, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& msa, const CUtensorMap& msb, cudaStream_t st) {
+static int launch_gemm8(Gemm8Args& g, const uint8_t* a, const CUtensorMap& mb, const CUtensorMap& msa, const CUtensorMap& msb, cudaStream_t st) {
     int dev = 0;
     cudaGetDevice(&dev);
     static bool configured[64] = {};
-    static int sm_count[64] = {};
+    static Slots slots[64] = {};
     NVFP4_REQUIRE(dev >= 0 && dev < 64, NVFP4_ERR_UNSUPPORTED, "nvfp4_fp8_gemm: device index above 63");
     if (!configured[dev]) {
         cudaError_t e = cudaFuncSetAttribute(fp8_gemm_kernel<TO>, cudaFuncAttributeMaxDynamicSharedMemorySize, pair8::SMEM);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_gemm_split_kernel<TO>, cudaFuncAttributeMaxDynamicSharedMemorySize, split8::SMEM);
-        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sm_count[dev], cudaDevAttrMultiProcessorCount, dev);
-        NVFP4_REQUIRE(e == cudaSuccess, NVFP4_ERR_LAUNCH, "nvfp4_fp8_gemm: cannot configure the kernels: %s", cudaGetErrorString(e));
+        // clusters do not fill every SM (a group of SMs holds whole clusters only): what the device says it runs at once
+        cudaLaunchConfig_t c = {};
+        cudaLaunchAttribute size[1];
+        size[0].id = cudaLaunchAttributeClusterDimension;
+        size[0].val.clusterDim.y = size[0].val.clusterDim.z = 1;
+        c.attrs = size;
+        c.numAttrs = 1;
+        for (int i = 0; i < 4 && e == cudaSuccess; ++i) {
+            size[0].val.clusterDim.x = 1 << i;
+            c.gridDim = dim3(8);
+            c.blockDim = dim3(split8::THREADS);
+            c.dynamicSmemBytes = split8::SMEM;
+            e = cudaOccupancyMaxActiveClusters(&slots[dev].clusters[i], fp8_gemm_split_kernel<TO>, &c);
+        }
+        if (e == cudaSuccess) {
+            size[0].val.clusterDim.x = 2;
+            c.blockDim = dim3(pair8::THREADS);
+            c.dynamicSmemBytes = pair8::SMEM;
+            e = cudaOccupancyMaxActiveClusters(&slots[dev].pairs, fp8_gemm_kernel<TO>, &c);
+        }
+        NVFP4_REQUIRE(e == cudaSuccess && slots[dev].pairs > 0, NVFP4_ERR_LAUNCH, "nvfp4_fp8_gemm: cannot configure the kernels: %s", cudaGetErrorString(e));
         configured[dev] = true;
     }
-    const int splits = split_for(g, sm_count[dev]);
+    const int splits = split_for(g, slots[dev]);
+    CUtensorMap ma;
+    NVFP4_REQUIRE(operand_map(&ma, a, g.M, g.k_tiles * static_cast<int64_t>(G8_BK), splits ? g.a_rows : 128), NVFP4_ERR_LAUNCH,
+                  "nvfp4_fp8_gemm: cuTensorMapEncodeTiled failed or is unavailable");
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -516,15 +555,15 @@ static int launch_gemm8(Gemm8Args& g, const CUtensorMap& ma, const CUtensorMap& 
     cfg.numAttrs = 1;
     cudaError_t e;
     if (splits == 0) {
-        CUtensorMap mo = ma;           // unused without tma_store, but the parameter must hold a valid map
-        constexpr int ESZ = sizeof(TO);
         g.tiles_m = (g.M + 255) / 256;
         g.tiles_n = (g.N + 255) / 256;
+        CUtensorMap mo = ma;           // unused without tma_store, but the parameter must hold a valid map
+        constexpr int ESZ = sizeof(TO);
         g.tma_store = aligned(g.out, 16) && g.ldo * ESZ % 16 == 0 &&
                       map_2d(&mo, ESZ == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, g.out, g.N, g.M, g.ldo * ESZ, 32 / ESZ, 32,
                              CU_TENSOR_MAP_SWIZZLE_32B);
         attr[0].val.clusterDim.x = 2;
-        cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min<int64_t>(static_cast<int64_t>(g.tiles_m) * g.tiles_n, sm_count[dev] / 2)));
+        cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min<int64_t>(static_cast<int64_t>(g.tiles_m) * g.tiles_n, slots[dev].pairs)));
         cfg.blockDim = dim3(pair8::THREADS);
         cfg.dynamicSmemBytes = pair8::SMEM;
         e = cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<TO>, ma, mb, msa, msb, mo, g);
@@ -560,14 +599,15 @@ extern "C" int nvfp4_fp8_gemm(const uint8_t* a, const uint8_t* a_scales, const u
         NVFP4_REQUIRE(aligned(p, 16), NVFP4_ERR_ALIGN, "nvfp4_fp8_gemm: operands and scales must be 16-byte aligned");
     NVFP4_REQUIRE(aligned(out, dtype_size(out_dtype)) && aligned(bias, bias ? dtype_size(bias_dtype) : 1), NVFP4_ERR_ALIGN,
                   "nvfp4_fp8_gemm: result and bias must be aligned to their elements");
-    Gemm8Args g{bias, out, status, ldo, bias_dtype, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K / 128), 0, 0, 0};
-    CUtensorMap ma, mb, msa, msb;
-    NVFP4_REQUIRE(operand_map(&ma, a, M, K) && operand_map(&mb, b, N, K) && scale_map(&msa, a_scales, M, K) && scale_map(&msb, b_scales, N, K),
+    Gemm8Args g{bias, out, status, ldo, bias_dtype, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K / 128), 0, 0, 0, 128};
+    g.a_rows = M < 128 ? static_cast<int>((M + 15) / 16 * 16) : 128;
+    CUtensorMap mb, msa, msb;
+    NVFP4_REQUIRE(operand_map(&mb, b, N, K, 128) && scale_map(&msa, a_scales, M, K) && scale_map(&msb, b_scales, N, K),
                   NVFP4_ERR_LAUNCH, "nvfp4_fp8_gemm: cuTensorMapEncodeTiled failed or is unavailable");
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (out_dtype == NVFP4_BF16) return launch_gemm8<__nv_bfloat16>(g, ma, mb, msa, msb, st);
-    if (out_dtype == NVFP4_F16) return launch_gemm8<__half>(g, ma, mb, msa, msb, st);
-    return launch_gemm8<float>(g, ma, mb, msa, msb, st);
+    if (out_dtype == NVFP4_BF16) return launch_gemm8<__nv_bfloat16>(g, a, mb, msa, msb, st);
+    if (out_dtype == NVFP4_F16) return launch_gemm8<__half>(g, a, mb, msa, msb, st);
+    return launch_gemm8<float>(g, a, mb, msa, msb, st);
 }
 
 extern "C" int64_t nvfp4_fp8_packing_bytes(int64_t rows, int64_t k) {
