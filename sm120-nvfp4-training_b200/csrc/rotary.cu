@@ -13,7 +13,9 @@
 namespace nvfp4 {
 
 constexpr int ROT_WARPS = 8;
-constexpr int ROT_AHEAD = 4;     // heads whose loads a lane has in flight
+// Heads whose loads a lane has in flight.  Three of them leave registers for three CTAs per SM: four (two CTAs) took 85 against
+// 78 us for 17408 tokens x 48 heads of 128 and 16.4 against 11.8 us for 3063 x 32 of 72 in FP32; two (four CTAs) took 79 and 11.9.
+constexpr int ROT_AHEAD = 3;
 
 struct RotaryArgs {
     const void* x[3];
@@ -42,7 +44,7 @@ __device__ __forceinline__ double position_at(const RotaryArgs& a, int64_t i) {
 // way (V divides pairs): V pairs (c V + i) in the split layout, V / 2 pairs of each vector in the interleaved one.  With
 // V == 1 the interleaved chunk is the two features 2c, 2c + 1.
 template <typename T, int V, bool INTER>
-__global__ void __launch_bounds__(ROT_WARPS * 32) rotary_axes_kernel(const __grid_constant__ RotaryArgs a) {
+__global__ void __launch_bounds__(ROT_WARPS * 32, 3) rotary_axes_kernel(const __grid_constant__ RotaryArgs a) {
     __shared__ float2 table[ROT_WARPS][NVFP4_ROTARY_MAX_PAIRS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int chunks = a.pairs / V;
