@@ -248,6 +248,14 @@ def status_word(device: torch.device) -> torch.Tensor:
     return buf
 
 
+def status_ptr(device: torch.device) -> int | None:
+    """Address of the device's status word, or None where a capture is open and the word does not exist yet: made there it
+    would live in the graph's memory and be zeroed by its replays."""
+    if device.index not in _STATUS and torch.cuda.is_current_stream_capturing():
+        return None
+    return status_word(device).data_ptr()
+
+
 def check_status(device=None) -> None:
     """Synchronising check of the device status words (tests, check_finite, end of a benchmark)."""
     for idx, buf in _STATUS.items():

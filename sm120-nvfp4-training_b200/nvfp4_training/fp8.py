@@ -93,7 +93,7 @@ def _forward(x, weight, bias, packed, need_x, need_w):
         with nat.on(dev):
             nat.check(nat.lib().nvfp4_fp8_linear(x2.data_ptr(), codes[x.dtype], m, k, pitch_of(x2), w.data_ptr(), w_code, n, w_pitch, nat.ptr(bias),
                                                  0 if bias is None else codes[bias.dtype], y.data_ptr(), work.data_ptr(), nat.ptr(x_t), nat.ptr(w_t),
-                                                 nat.status_word(dev).data_ptr(), nat.raw_stream(dev)))
+                                                 nat.status_ptr(dev), nat.raw_stream(dev)))
     return y, x_t, (packed.packing_t if weight is None else w_t)
 
 
@@ -127,7 +127,7 @@ class _Fp8Linear(torch.autograd.Function):
         with nat.on(dev):
             nat.check(nat.lib().nvfp4_fp8_linear_bwd(g.data_ptr(), codes[g.dtype], m, n, k, pitch_of(g), nat.ptr(x_t), nat.ptr(w_t), nat.ptr(dx), nat.ptr(dw),
                                                      0 if dw is None else codes[dw.dtype], nat.ptr(db), 0 if db is None else codes[b_dtype],
-                                                     work.data_ptr(), nat.status_word(dev).data_ptr(), nat.raw_stream(dev)))
+                                                     work.data_ptr(), nat.status_ptr(dev), nat.raw_stream(dev)))
         if taken is not None:
             taken(dw)
             dw = None

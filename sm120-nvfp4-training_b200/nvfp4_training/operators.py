@@ -72,7 +72,7 @@ def _norm_forward(x, delta, weight, bias, eps, out_dtype, amax, keep_stats):
                 x2.data_ptr(), codes[x.dtype], pitch_of(x2), nat.ptr(d2), 0 if d2 is None else codes[d2.dtype], 0 if d2 is None else pitch_of(d2),
                 nat.ptr(weight), nat.ptr(bias), 0 if affine is None else codes[affine.dtype], eps, rows, cols,
                 None if d2 is None else total.data_ptr(), h.data_ptr(), codes[out_dtype], at, at and at + 4 * rows, nat.ptr(amax),
-                nat.status_word(dev).data_ptr(), nat.raw_stream(dev)))
+                nat.status_ptr(dev), nat.raw_stream(dev)))
     return total, h, stats
 
 
@@ -120,7 +120,7 @@ class _LayerNorm(torch.autograd.Function):
                     g.data_ptr(), codes[g.dtype], pitch_of(g), total.data_ptr(), codes[total.dtype], pitch_of(total), at, at + 4 * rows,
                     nat.ptr(weight), 0 if wdtype is None else codes[wdtype], nat.ptr(res), 0 if res is None else pitch_of(res), rows, cols,
                     dx.data_ptr(), nat.ptr(dd), nat.ptr(partial), nat.ptr(dw), nat.ptr(db), nat.ptr(amax),
-                    nat.status_word(dev).data_ptr(), nat.raw_stream(dev)))
+                    nat.status_ptr(dev), nat.raw_stream(dev)))
         else:
             for t in (dw, db):
                 if t is not None:
@@ -305,6 +305,8 @@ def _check_rotary(x, batch, seq, dim, positions, sections, theta, layout, freque
     how = _plan(tuple(sections), dim, float(theta), layout, frequencies)
     _check_tensor("positions", positions, _POSITION_KINDS)
     shape = positions.shape
+    if positions.requires_grad:
+        raise ValueError("positions have no gradient here; pass them detached")
     if positions.device != x.device or shape[-2:] != (seq, how[1]) or not (len(shape) == 2 or (len(shape) == 3 and shape[0] == batch)):
         raise ValueError(f"positions must be [{seq}, {how[1]}] or [{batch}, {seq}, {how[1]}] on the input's device")
     _check_device(x)

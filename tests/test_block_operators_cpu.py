@@ -60,6 +60,7 @@ Q, POS = x(2, 5, 4, 16), torch.zeros(5, 2, dtype=torch.int64)
     (ValueError, lambda: nv.rotary_axes(Q, Q, POS, (3, 5), theta=float("inf"))),
     (TypeError, lambda: nv.rotary_axes(Q, Q, POS.to(torch.int16), (3, 5))),
     (ValueError, lambda: nv.rotary_axes(Q, Q, torch.zeros(3, 5, 2, dtype=torch.int64), (3, 5))),
+    (ValueError, lambda: nv.rotary_axes(Q, Q, POS.float().requires_grad_(True), (3, 5))),
     (ValueError, lambda: nv.rotary_axes(Q, Q, POS, (3, 5))),                         # CPU tensors
     (ValueError, lambda: nv.rotary_axes_qkv(x(2, 5, 50), POS, (3, 5), 4)),           # 50 is not 12 heads of anything
     (ValueError, lambda: nv.rotary_axes_qkv(x(2, 5, 4, 48), POS, (3, 5), 4)),
