@@ -75,14 +75,19 @@ __global__ void __launch_bounds__(F8_THREADS, Fp8Map<T>::CTAS) fp8_quantize_kern
     const int cl = lane % L, part = lane / L;                 // column group, and which run of I rows of the warp's sixteen
     const int row_in = warp * 16 + part * I, col_in = cl * E;
     const int64_t row0 = rb * 128 + row_in, col0 = cb * 128 + col_in;
+    const int rows_left = static_cast<int>(min(max(a.rows - row0, static_cast<int64_t>(0)), static_cast<int64_t>(I)));
 
     Pack<T, E> v[I];
     const T* src = static_cast<const T*>(a.x) + row0 * a.pitch + col0;
     const bool whole = a.vector && col0 + E <= a.cols;
+    if (whole && rows_left == I) {
 #pragma unroll
-    for (int i = 0; i < I; ++i) {
-        v[i] = Pack<T, E>{};
-        if (row0 + i < a.rows) {
+        for (int i = 0; i < I; ++i) v[i] = load_pack<T, E>(src + i * a.pitch);
+    } else {
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            v[i] = Pack<T, E>{};
+            if (i >= rows_left) continue;
             if (whole) v[i] = load_pack<T, E>(src + i * a.pitch);
             else {
 #pragma unroll
@@ -169,15 +174,15 @@ __global__ void __launch_bounds__(F8_THREADS, Fp8Map<T>::CTAS) fp8_quantize_kern
         }
     }
     if (a.codes) {
+        uint8_t* out = a.codes + row0 * a.cols_p + col0;
 #pragma unroll
-        for (int i = 0; i < I; ++i) {
+        for (int i = 0; i < I; ++i, out += a.cols_p) {
             const float inverse = SQUARE ? square.inverse : row_inverse[row_in + i];
             float f[E];
             unpack(v[i], f);
 #pragma unroll
             for (int j = 0; j < E; ++j) f[j] *= inverse;
-            if (row0 + i < a.rows) {
-                uint8_t* out = a.codes + (row0 + i) * a.cols_p + col0;
+            if (i < rows_left) {
                 if constexpr (E == 8) *reinterpret_cast<uint2*>(out) = make_uint2(e4m3x4(f[0], f[1], f[2], f[3]), e4m3x4(f[4], f[5], f[6], f[7]));
                 else *reinterpret_cast<uint32_t*>(out) = e4m3x4(f[0], f[1], f[2], f[3]);
             }
@@ -215,12 +220,13 @@ __global__ void __launch_bounds__(F8_THREADS, Fp8Map<T>::CTAS) fp8_quantize_kern
             }
         }
         __syncthreads();
+        const int first = warp * 2 + (lane >> 4), piece = lane & 15;
+        const int cols_left = static_cast<int>(min(a.cols - cb * 128, static_cast<int64_t>(128))) - first;
+        uint8_t* out = a.codes_t + (cb * 128 + first) * a.rows_p + rb * 128 + piece * 8;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int c = k * 16 + warp * 2 + (lane >> 4), piece = lane & 15;
-            if (cb * 128 + c < a.cols)
-                *reinterpret_cast<uint2*>(a.codes_t + (cb * 128 + c) * a.rows_p + rb * 128 + piece * 8) =
-                    *reinterpret_cast<const uint2*>(turned + c * 128 + ((piece ^ (c >> 3)) & 15) * 8);
+        for (int k = 0; k < 8; ++k, out += 16 * a.rows_p) {
+            const int c = k * 16 + first;
+            if (k * 16 < cols_left) *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(turned + c * 128 + ((piece ^ (c >> 3)) & 15) * 8);
         }
     }
 }

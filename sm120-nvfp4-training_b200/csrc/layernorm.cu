@@ -368,23 +368,27 @@ __global__ void __launch_bounds__(256) norm_bwd_columns_kernel(const NormBwdArgs
 }
 
 // out[c] = sum of `parts` rows of `width` floats, columns [0, cols) to out0 and [cols, 2 cols) to out1 (either may be null).
-// A CTA takes 32 columns, its 32 warps every 32nd row each, the subtotals are added in warp order.
-__global__ void __launch_bounds__(1024) column_sums_kernel(const float* __restrict__ partial, int64_t parts, int64_t width, int64_t cols,
-                                                           void* out0, void* out1, int dtype) {
-    __shared__ float subtotal[32][33];
+// A CTA takes 32 columns, its 16 warps every 16th row each, the subtotals are added in warp order.  (32 warps a CTA leave a
+// second wave of CTAs at 2 * 5120 columns.)
+constexpr int SUM_WARPS = 16;
+__global__ void __launch_bounds__(SUM_WARPS * 32) column_sums_kernel(const float* __restrict__ partial, int64_t parts, int64_t width, int64_t cols,
+                                                                     void* out0, void* out1, int dtype) {
+    __shared__ float subtotal[SUM_WARPS][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
     float t = 0.f;
     if (c < width) {
 #pragma unroll 8
-        for (int64_t p = warp; p < parts; p += 32) t += partial[p * width + c];
+        for (int64_t p = warp; p < parts; p += SUM_WARPS) t += partial[p * width + c];
     }
     subtotal[warp][lane] = t;
     __syncthreads();
-    const int64_t mine = static_cast<int64_t>(blockIdx.x) * 32 + warp;        // a warp adds one column's subtotals
-    t = warp_sum(subtotal[lane][warp]);
-    void* out = mine < cols ? out0 : out1;
-    if (lane == 0 && mine < width && out) store_param(out, dtype, mine < cols ? mine : mine - cols, t);
+    if (warp != 0 || c >= width) return;
+    t = 0.f;
+#pragma unroll
+    for (int w = 0; w < SUM_WARPS; ++w) t += subtotal[w][lane];
+    void* out = c < cols ? out0 : out1;
+    if (out) store_param(out, dtype, c < cols ? c : c - cols, t);
 }
 
 // ====================================================================================================================
@@ -970,14 +974,14 @@ extern "C" int nvfp4_layer_norm_bwd(const void* dh, int h_dtype, int64_t dh_pitc
     else if (h_dtype == NVFP4_F32) parts = backward<float, float>(a, vector, ring, st);
     else parts = backward<float, __nv_bfloat16>(a, vector, ring, st);
     if (a.partial)
-        column_sums_kernel<<<static_cast<unsigned>((2 * cols + 31) / 32), 1024, 0, st>>>(partial, parts, 2 * cols, cols, dweight, dbias, weight_dtype);
+        column_sums_kernel<<<static_cast<unsigned>((2 * cols + 31) / 32), SUM_WARPS * 32, 0, st>>>(partial, parts, 2 * cols, cols, dweight, dbias, weight_dtype);
     return launch_status("nvfp4_layer_norm_bwd");
 }
 
 extern "C" int nvfp4_column_sums(const float* partial, int64_t parts, int64_t cols, void* out, int out_dtype, nvfp4_stream_t stream) {
     NVFP4_REQUIRE(partial && out && parts > 0 && cols > 0 && cols < (1LL << 31), NVFP4_ERR_ARG, "nvfp4_column_sums: null pointer or empty size");
     NVFP4_REQUIRE(is_float_dtype(out_dtype), NVFP4_ERR_DTYPE, "nvfp4_column_sums: FP32, BF16 or FP16 result");
-    column_sums_kernel<<<static_cast<unsigned>((cols + 31) / 32), 1024, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+    column_sums_kernel<<<static_cast<unsigned>((cols + 31) / 32), SUM_WARPS * 32, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
         partial, parts, cols, cols, out, nullptr, out_dtype);
     return launch_status("nvfp4_column_sums");
 }
