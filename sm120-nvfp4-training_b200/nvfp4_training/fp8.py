@@ -16,7 +16,7 @@ import torch
 from torch import nn
 
 from . import _native as nat
-from .operators import _check_device, _check_tensor, pitch_of, rows_of
+from .operators import _check_device, _check_tensor, _once, pitch_of, rows_of
 
 _MAX = 1 << 30
 
@@ -54,16 +54,16 @@ class PackedFP8:
         return (codes.view(torch.float8_e4m3fn).double() * scale)[:, :cols].float()
 
 
-def _bytes(n, device):
-    return torch.empty(n, dtype=torch.uint8, device=device)
+def _bytes(n, beside):
+    return beside.new_empty(n, dtype=torch.uint8)
 
 
 def _quantize(x, *, row, col, square=False, column_sums=False):
     """(packing or None, transposed packing or None, FP32 partial column sums or None) of x [rows, cols]."""
     rows, cols = x.shape
     dev = x.device
-    a = _bytes(_packing_bytes(rows, cols), dev) if row else None
-    t = _bytes(_packing_bytes(cols, rows), dev) if col else None
+    a = _bytes(_packing_bytes(rows, cols), x) if row else None
+    t = _bytes(_packing_bytes(cols, rows), x) if col else None
     sums = torch.empty((_ceil128(rows), cols), dtype=torch.float32, device=dev) if column_sums else None
     at, tt = nat.ptr(a), nat.ptr(t)
     with nat.on(dev):
@@ -83,13 +83,13 @@ def _forward(x, weight, bias, packed, need_x, need_w):
         n, k = weight.shape
         w = rows_of(weight, k)
         w_code, w_pitch, w_bytes = codes[w.dtype], pitch_of(w), _packing_bytes(n, k)
-        w_t = _bytes(_packing_bytes(k, n), dev) if need_x else None
+        w_t = _bytes(_packing_bytes(k, n), x) if need_x else None
     x2 = rows_of(x, k)
     m = x2.shape[0]
-    y = torch.empty((m, n) if x.ndim == 2 else (*x.shape[:-1], n), dtype=x.dtype, device=dev)
-    x_t = _bytes(_packing_bytes(k, m), dev) if need_w else None
+    y = x.new_empty((m, n) if x.ndim == 2 else (*x.shape[:-1], n))
+    x_t = _bytes(_packing_bytes(k, m), x) if need_w else None
     if m:
-        work = _bytes(_packing_bytes(m, k) + w_bytes, dev)
+        work = _bytes(_packing_bytes(m, k) + w_bytes, x)
         with nat.on(dev):
             nat.check(nat.lib().nvfp4_fp8_linear(x2.data_ptr(), codes[x.dtype], m, k, pitch_of(x2), w.data_ptr(), w_code, n, w_pitch, nat.ptr(bias),
                                                  0 if bias is None else codes[bias.dtype], y.data_ptr(), work.data_ptr(), nat.ptr(x_t), nat.ptr(w_t),
@@ -110,18 +110,18 @@ class _Fp8Linear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, grad):
         m, n, k, need_x, need_w, b_dtype, shape, dtype = ctx.how
         weight, w_t, x_t = ctx.saved_tensors
         dev = grad.device
-        dx = torch.empty(shape, dtype=dtype, device=dev) if need_x else None
-        db = None if b_dtype is None else torch.empty(n, dtype=b_dtype, device=dev)
+        dx = grad.new_empty(shape, dtype=dtype) if need_x else None
+        db = None if b_dtype is None else grad.new_empty(n, dtype=b_dtype)
         if not m:
             return dx, (torch.zeros(weight.shape, dtype=weight.dtype, device=dev) if need_w else None), (None if db is None else db.zero_()), None
         dw, taken = _weight_gradient_into(weight) if need_w else (None, None)
         columns = need_w or db is not None
-        work = _bytes((_packing_bytes(m, n) if need_x else 0) + (_packing_bytes(n, m) + 4 * n * _ceil128(m) if columns else 0), dev)
+        work = _bytes((_packing_bytes(m, n) if need_x else 0) + (_packing_bytes(n, m) + 4 * n * _ceil128(m) if columns else 0), grad)
         g = rows_of(grad, n)
         codes = nat._CODES
         with nat.on(dev):
@@ -137,7 +137,7 @@ class _Fp8Linear(torch.autograd.Function):
 def _weight_gradient_into(weight):
     """(tensor that receives dW, None), or with a function that hands it on where an optimizer collects gradients itself
     (backward_step, captured steps) instead of autograd."""
-    new = lambda dtype: torch.empty(weight.shape, dtype=dtype, device=weight.device)
+    new = lambda dtype: torch.empty_like(weight, dtype=dtype, memory_format=torch.contiguous_format)
     sink = getattr(weight, "_v4_pending", None)
     if sink is None or weight.numel() < 4096:          # smaller weights have FP32 moments and take an ordinary gradient
         return new(weight.dtype), None

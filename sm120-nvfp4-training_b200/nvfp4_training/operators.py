@@ -51,6 +51,21 @@ def pitch_of(flat):
     return max(flat.stride(0), flat.shape[1])
 
 
+def _like(t):
+    """A new contiguous tensor of t's shape and dtype (empty_like is the cheapest way to one, but copies strides)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
+def _once(impl):
+    """torch.autograd.function.once_differentiable, entered only where a second derivative could be asked for: outside
+    create_graph=True backward runs without gradients anyway, and the wrapper is host time of every small call."""
+    checked = torch.autograd.function.once_differentiable(impl)
+
+    def backward(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else impl(ctx, *grads)
+    return backward
+
+
 def _norm_forward(x, delta, weight, bias, eps, out_dtype, amax, keep_stats):
     """(total [rows, cols], h, statistics or None): h and a new total in x's shape, total as rows."""
     shape, dev = x.shape, x.device
@@ -60,9 +75,9 @@ def _norm_forward(x, delta, weight, bias, eps, out_dtype, amax, keep_stats):
     d2, total = None, x2
     if delta is not None:
         d2 = rows_of(delta, cols)
-        total = torch.empty((rows, cols), dtype=x.dtype, device=dev)
-    h = torch.empty(shape, dtype=out_dtype, device=dev)
-    stats = torch.empty(2 * rows, dtype=torch.float32, device=dev) if keep_stats else None
+        total = _like(x2)
+    h = _like(x) if out_dtype == x.dtype else x.new_empty(shape, dtype=out_dtype)
+    stats = x.new_empty(2 * rows, dtype=torch.float32) if keep_stats else None
     if rows:
         at = stats.data_ptr() if keep_stats else None
         affine = weight if weight is not None else bias
@@ -89,10 +104,10 @@ class _LayerNorm(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         if amax is not None:
             ctx.mark_non_differentiable(amax)
-        return (None if delta is None else total.view(x.shape)), h, amax
+        return (None if delta is None else total if x.ndim == 2 else total.view(x.shape)), h, amax
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dsum, dh, _):
         total, stats, weight = ctx.saved_tensors
         rows, cols = total.shape
@@ -104,16 +119,17 @@ class _LayerNorm(torch.autograd.Function):
             return dsum, dd, (zero if need_w else None), (zero if need_b else None), None, None, None
         g = rows_of(dh, cols)
         res = None if dsum is None else rows_of(dsum, cols)
-        dx = torch.empty(ctx.shape, dtype=total.dtype, device=dev)
+        flat = len(ctx.shape) == 2
+        dx = _like(total) if flat else total.new_empty(ctx.shape)
         narrow = ctx.delta_dtype is not None and ctx.delta_dtype != total.dtype
-        dd = torch.empty(ctx.shape, dtype=ctx.delta_dtype, device=dev) if narrow else None
-        dw = torch.empty(cols, dtype=wdtype, device=dev) if need_w else None
-        db = torch.empty(cols, dtype=wdtype, device=dev) if need_b else None
+        dd = total.new_empty(ctx.shape, dtype=ctx.delta_dtype) if narrow else None
+        dw = torch.empty_like(weight) if need_w else None
+        db = None if not need_b else torch.empty_like(dw) if need_w else total.new_empty(cols, dtype=wdtype)
         amax = _zeroed_slot(dev) if ctx.want_amax and (narrow or total.dtype == torch.bfloat16) else None
         if rows:
             lib, partial, codes = nat.lib(), None, nat._CODES
             if need_w or need_b:
-                partial = torch.empty(lib.nvfp4_layer_norm_bwd_partials(rows, cols) * 2 * cols, dtype=torch.float32, device=dev)
+                partial = stats.new_empty(lib.nvfp4_layer_norm_bwd_partials(rows, cols) * 2 * cols)
             at = stats.data_ptr()
             with nat.on(dev):
                 nat.check(lib.nvfp4_layer_norm_bwd(
@@ -160,7 +176,7 @@ def _layer_norm(x, delta, weight, bias, eps, out_dtype, want_amax=False):
     if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, delta, weight, bias))):
         amax = _zeroed_slot(x.device) if want_amax and out_dtype == torch.bfloat16 else None
         total, h, _ = _norm_forward(x, delta, weight, bias, eps, out_dtype, amax, False)
-        return (None if delta is None else total.view(x.shape)), h, amax
+        return (None if delta is None else total if x.ndim == 2 else total.view(x.shape)), h, amax
     return _LayerNorm.apply(x, delta, weight, bias, eps, out_dtype, want_amax and out_dtype == torch.bfloat16)
 
 
@@ -243,7 +259,7 @@ def _features_contiguous(t):
 
 def _turn(tensors, positions, how, inverse):
     """Rotated copies of the tensors that are not None, in one launch."""
-    outs = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in tensors]
+    outs = [None if t is None else _like(t) for t in tensors]
     jobs = [(_features_contiguous(t), o, 1) for t, o in zip(tensors, outs) if t is not None and t.numel()]
     if jobs:
         _launch_rotary(jobs, positions, *how, inverse, None)
@@ -259,7 +275,7 @@ class _RotaryAxes(torch.autograd.Function):
         return tuple(_turn((q, k), positions, how, False))
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dq, dk):
         positions, = ctx.saved_tensors
         return (*_turn((dq, dk), positions, ctx.how, True), None, None)
@@ -283,12 +299,12 @@ class _RotaryFused(torch.autograd.Function):
         return (*_turn((q, k), positions, how, False), v)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dq, dk, dv):
         positions, = ctx.saved_tensors
         shape, heads, kv_heads = ctx.dims
         some = next(g for g in (dq, dk, dv) if g is not None)
-        dqkv = torch.empty(shape, dtype=some.dtype, device=some.device)
+        dqkv = some.new_empty(shape)
         amax = _zeroed_slot(some.device) if some.dtype == torch.bfloat16 else None
         jobs = []
         for g, o, turn in zip((dq, dk, dv), _split_heads(dqkv, heads, kv_heads), (1, 1, 0)):

@@ -266,3 +266,13 @@ def test_widths_around_the_kernels_borders(cols, rows, dtype, delta_dtype):
         check(got, want, scale, "gradients")
     from nvfp4_training import _native
     _native.check_status()
+
+
+def test_second_derivatives_are_refused_where_they_would_pass_through():
+    x = torch.randn(4, 64, device="cuda", requires_grad=True)
+    pos = torch.arange(4, device="cuda").view(1, 4, 1)
+    w = torch.randn(64, 64, device="cuda", requires_grad=True)
+    for y in (nv.layer_norm(x), nv.rotary_axes(x.view(1, 4, 1, 64), None, pos, (32,))[0], nv.fp8_linear(x, w)):
+        dx, = torch.autograd.grad((y * y).sum(), x, create_graph=True)       # first derivatives with a graph are fine
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(dx.sum(), x)
