@@ -9,7 +9,9 @@
 // row of the tile is a 1 x 128 block, a column of it a transposed block and the tile a square block; the whole tile is in
 // registers after one round of loads (32 KB in flight per CTA), eight rows of one 16-byte column group per lane.  Row codes go
 // straight out (128-byte segments); transposed codes pass through shared memory as 8-byte pieces (eight rows of a column),
-// placed with their index exclusive-ored by the column group so that neither side has bank conflicts.
+// placed with their index exclusive-ored by the column group so that neither side has bank conflicts.  Both packings of
+// 16384 x 14336 BF16 take 162 us (0.90 of the measured HBM rate), the row packing alone 107 us (1.0); of 8192 x 4096 28 us
+// (0.74: 3.5 waves of tiles), of such a weight in 128 x 128 blocks 23.5 us (0.89).
 #include "bf16x8.cuh"
 #include "vec.cuh"
 
