@@ -281,3 +281,24 @@ def test_every_layer_at_8_bits():
         losses = [graph.step(x, y).item() for _ in range(3)]
     nv.check_finite(model)
     assert all(l == l for l in losses)
+
+
+def test_data_parallel_slots_of_one_rank(tmp_path):
+    """One rank of a data-parallel job: the 8-bit layers write their gradients into the reducer's slots, and with one rank the
+    updates are those of the model without it."""
+    import torch.distributed as dist
+    x, y = batch()
+
+    def all_fp8():
+        torch.manual_seed(3)
+        return nv.enable_nvfp4(Model(), profile="balanced", lr=1e-3, fp8_layers=["*"])
+    alone = all_fp8()
+    want = [nv.train_step(alone, loss_fn, x, y).item() for _ in range(3)]
+    dist.init_process_group("gloo", init_method=f"file://{tmp_path}/store", rank=0, world_size=1)
+    try:
+        model = nv.enable_data_parallel(all_fp8())
+        assert model.nvfp4_optimizer.reducer.has_slot(model.up.weight)
+        assert [nv.train_step(model, loss_fn, x, y).item() for _ in range(3)] == want
+        assert all(torch.equal(a, b) for a, b in zip(model.parameters(), alone.parameters()))
+    finally:
+        dist.destroy_process_group()

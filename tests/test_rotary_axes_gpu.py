@@ -170,3 +170,26 @@ def test_streams_graphs_and_repeats():
     again = nv.rotary_axes_qkv(leaf, pos, (8, 8), 4)
     assert all(torch.equal(a, b) for a, b in zip(outs, again))
     assert torch.equal(grad, torch.autograd.grad(again, leaf, (dq, dq, dq))[0])
+
+
+def test_in_place_edits_do_not_go_unseen():
+    """v is a view of the projection: writing to it either is refused or counts in the gradients."""
+    g = torch.Generator(device="cuda").manual_seed(12)
+    qkv = rand(g, 1, 6, 12 * 16).requires_grad_(True)
+    pos = positions(g, 1, 6, 1)
+    q, k, v = nv.rotary_axes_qkv(qkv * 1.0, pos, (8,), 4)
+    try:
+        v.mul_(2)
+    except RuntimeError:
+        return
+    grad, = torch.autograd.grad(v.sum(), qkv)
+    assert torch.equal(grad.view(1, 6, 12, 16)[:, :, 8:], torch.full((1, 6, 4, 16), 2.0, device="cuda"))
+
+
+def test_edited_positions_are_noticed():
+    q = torch.randn(1, 4, 1, 16, device="cuda", requires_grad=True)
+    pos = torch.arange(4, device="cuda").view(4, 1)
+    out, _ = nv.rotary_axes(q, None, pos, (8,))
+    pos.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        out.sum().backward()
