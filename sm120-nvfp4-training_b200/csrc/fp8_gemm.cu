@@ -1,8 +1,9 @@
 // Products of e4m3 operands with a power-of-two scale per block of 128:  out[M][N] = (A o SA) (B o SB)^T (+ bias).
 //
 // tcgen05.mma.kind::mxf8f6f4 multiplies a UE8M0 scale into every 32 elements of the contraction; the packings give the four
-// 32-blocks of a 128-block the same byte, so the tensor cores apply the block scale themselves and accumulate over the whole
-// contraction in FP32 tensor memory, without a pass of multiply-adds per block on the CUDA cores.
+// 32-blocks of a 128-block the same byte, so the tensor cores apply the block scale themselves and accumulate in FP32 tensor
+// memory, over the whole contraction for a 16-bit result (CHUNK below has the rule for FP32 ones), without a pass of
+// multiply-adds per block on the CUDA cores.
 //
 // Two kernels.
 //   fp8_gemm_kernel        persistent clusters of two CTAs on 256 x 256 tiles (cta_group::2, M256 x N256 x K32 instructions), for
@@ -23,12 +24,23 @@
 #include "vec.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace nvfp4 {
 
 constexpr int G8_BK = 128;                  // elements (and bytes) of the contraction per stage: one scale block
 constexpr int G8_SF = 512;                  // bytes of a scale block: 128 rows x 4
 constexpr int G8_OPERAND = 128 * 128;       // bytes of 128 rows of an operand per stage
+
+// The tensor cores drop bits towards zero when they add to an accumulator, so a sum of terms of one sign falls behind steadily
+// (measured relative error of the paired kernel, positive operands: 5e-7 after 2048 elements, 1.4e-6 after 4096, 9.9e-6 after
+// 16384, 1.05e-4 after 66000; signs that cancel: 1.1e-7, 2.2e-7, 1.2e-6 after 16384).  A 16-bit result is itself rounded by 2e-3
+// (BF16) or 5e-4 (FP16) and keeps the one accumulator.  For FP32 results
+// the accumulator is emptied into FP32 registers every CHUNK k-tiles (2048 elements): 5e-7 (1.2e-7) whatever the length.  Between
+// chunks the tensor cores wait about 0.6 us for the epilogue: 14336 x 4096 x 8192 341 -> 364 us, 8192 x 4096 x 4096 100 -> 106;
+// up to 2048 elements nothing.  Chunks of 1024 bring 1.9e-7 and cost 14 to 20 %; of 4096, 1.4e-6 and 4 to 5 %.
+constexpr int CHUNK = 16;
+template <typename TO> struct Chunked { static constexpr bool value = sizeof(TO) == 4; };
 
 struct Gemm8Args {
     const void* bias;
@@ -83,9 +95,11 @@ constexpr int STAGE_BYTES = OPERANDS + SCALES;
 // Tensor memory: two accumulators of 256 columns that share 32 ([0, 256) and [224, 480)), so that two scale buffers of
 // 4 + 8 columns fit behind them.  The epilogue reads the shared columns first, and only that read gates the next tile.
 constexpr int ACC_STRIDE = 224, SF_BASE = 480, SF_COLS = 12, TMEM_COLS = 512;
-constexpr int SLAB = 1024;                           // 32 rows x 32 bytes, two per epilogue warp
+// Staging of an epilogue warp: units of 32 rows x 16 columns, two of 16-bit results or one of FP32.  (FP32 as two boxes 32 bytes
+// wide was slower, 4096 x 4096 x 1024 30.7 against 26.7 us; five load stages and two or three units were no faster.)
+constexpr int STAGING = 2048;
 constexpr int BARS = 2 * STAGES + 4;
-constexpr int SMEM = STAGES * STAGE_BYTES + EPI_WARPS * 2 * SLAB + 1024 + 256;
+constexpr int SMEM = STAGES * STAGE_BYTES + EPI_WARPS * STAGING + 1024 + 256;
 static_assert(SF_BASE + 2 * SF_COLS <= TMEM_COLS && BARS * 8 + 16 <= 256 && SMEM <= 232448, "budgets");
 }  // namespace pair8
 
@@ -97,7 +111,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* epi_smem = smem + STAGES * OPERANDS;
-    uint8_t* sf_smem = epi_smem + EPI_WARPS * 2 * SLAB;
+    uint8_t* sf_smem = epi_smem + EPI_WARPS * STAGING;
     uint64_t* full = reinterpret_cast<uint64_t*>(sf_smem + STAGES * SCALES);
     uint64_t* empty = full + STAGES;
     uint64_t* acc_full = empty + STAGES;
@@ -170,117 +184,148 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             int stage = 0, local = 0, sf_buf = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (int t = first_tile; t < total_tiles && ok; t += tile_step, ++local) {
-                const int acc = local & 1;
-                const uint32_t tmem_acc = tmem_base + acc * ACC_STRIDE;
-                if (local > 0) {       // the previous tile's shared columns are read, and with them everything of the tile before
-                    if (!mbar_wait_warp(shared_drained, (local - 1) & 1, abort_flag)) { ok = false; break; }
-                    tc_fence_after();
-                }
-                for (int kt = 0; kt < g.k_tiles; ++kt) {
-                    if (!mbar_wait_warp(&full[stage], phase, abort_flag)) { ok = false; break; }
-                    tc_fence_after();
-                    if (elect_one()) {
-                        const uint32_t sa = smem_u32(smem + stage * OPERANDS), sb = sa + G8_OPERAND, sf = smem_u32(sf_smem + stage * SCALES);
-                        const uint32_t tsfa = tmem_base + SF_BASE + sf_buf * SF_COLS, tsfb = tsfa + 4;
-                        tc_cp_sf_pair(tsfa, scale_desc(sf));
-                        tc_cp_sf_pair(tsfb, scale_desc(sf + G8_SF));
-                        tc_cp_sf_pair(tsfb + 4, scale_desc(sf + 2 * G8_SF));
-#pragma unroll
-                        for (int kb = 0; kb < 4; ++kb)
-                            mma8<true>(tmem_acc, operand_desc(sa + kb * 32), operand_desc(sb + kb * 32), idesc, (kt | kb) ? 1u : 0u, tsfa, tsfb);
-                        tc_commit_pair(&empty[stage]);
+            for (int t = first_tile; t < total_tiles && ok; t += tile_step) {
+                for (int k0 = 0, k1; k0 < g.k_tiles && ok; k0 = k1, ++local) {       // a chunk, or the whole contraction
+                    k1 = Chunked<TO>::value ? min(k0 + CHUNK, g.k_tiles) : g.k_tiles;
+                    const int acc = local & 1;
+                    const uint32_t tmem_acc = tmem_base + acc * ACC_STRIDE;
+                    if (local > 0) {       // the shared columns of the one before are read, and with them everything of the one before that
+                        if (!mbar_wait_warp(shared_drained, (local - 1) & 1, abort_flag)) { ok = false; break; }
+                        tc_fence_after();
                     }
+                    for (int kt = k0; kt < k1; ++kt) {
+                        if (!mbar_wait_warp(&full[stage], phase, abort_flag)) { ok = false; break; }
+                        tc_fence_after();
+                        if (elect_one()) {
+                            const uint32_t sa = smem_u32(smem + stage * OPERANDS), sb = sa + G8_OPERAND, sf = smem_u32(sf_smem + stage * SCALES);
+                            const uint32_t tsfa = tmem_base + SF_BASE + sf_buf * SF_COLS, tsfb = tsfa + 4;
+                            tc_cp_sf_pair(tsfa, scale_desc(sf));
+                            tc_cp_sf_pair(tsfb, scale_desc(sf + G8_SF));
+                            tc_cp_sf_pair(tsfb + 4, scale_desc(sf + 2 * G8_SF));
+#pragma unroll
+                            for (int kb = 0; kb < 4; ++kb)
+                                mma8<true>(tmem_acc, operand_desc(sa + kb * 32), operand_desc(sb + kb * 32), idesc, (kt > k0 || kb) ? 1u : 0u, tsfa, tsfb);
+                            tc_commit_pair(&empty[stage]);
+                        }
+                        __syncwarp();
+                        sf_buf ^= 1;
+                        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+                    }
+                    if (ok && elect_one()) tc_commit_pair(&acc_full[acc]);
                     __syncwarp();
-                    sf_buf ^= 1;
-                    if (++stage == STAGES) { stage = 0; phase ^= 1; }
                 }
-                if (ok && elect_one()) tc_commit_pair(&acc_full[acc]);
-                __syncwarp();
             }
         }
     } else {
         // ---- epilogue: two warps per TMEM sub-partition, eight 16-column units of the tile each ----
-        constexpr int ESZ = sizeof(TO);
+        constexpr int ESZ = sizeof(TO), SLAB = 32 * 16 * ESZ, SLABS = STAGING / SLAB;
         const int sub = warp & 3, half = (warp - FIRST_EPI_WARP) >> 2;
-        uint8_t* slabs = epi_smem + (warp - FIRST_EPI_WARP) * 2 * SLAB;
+        uint8_t* slabs = epi_smem + (warp - FIRST_EPI_WARP) * STAGING;
         int local = 0, turn = 0;
-        // 32 rows x 32 bytes, two uint4 per lane: through one of two staging slabs and a TMA store (which crops), or directly.
+        // A unit: 32 rows x 16 columns, a row per lane, through a staging slab and a TMA store (which crops), or directly.
         // (Each lane storing its row's 32 bytes itself was slower wherever tiles end together: 4304 x 1152 x 1000 17.5 against 13.8 us.)
-        auto emit = [&](const uint4& q0, const uint4& q1, int64_t row, int64_t col0, int tile_row0) {
+        auto emit = [&](const uint32_t (&w)[4 * ESZ], int64_t row, int64_t col0, int tile_row0) {
             if (g.tma_store) {
-                uint8_t* slab = slabs + (turn ^= SLAB);
-                if (lane == 0) bulk_wait_read<1>();      // the store before the last has read this slab
+                uint8_t* slab = slabs + turn * SLAB;
+                turn = turn + 1 == SLABS ? 0 : turn + 1;
+                if (lane == 0) bulk_wait_read<SLABS - 1>();      // the store that last used this slab has read it
                 __syncwarp();
-                const int sw = (lane >> 2) & 1;
-                *reinterpret_cast<uint4*>(slab + lane * 32 + (sw << 4)) = q0;
-                *reinterpret_cast<uint4*>(slab + lane * 32 + ((1 ^ sw) << 4)) = q1;
+                const int sw = (lane >> (ESZ == 2 ? 2 : 1)) & (ESZ - 1);      // the map's swizzle: 16-byte pieces by row, free of bank conflicts
+#pragma unroll
+                for (int c = 0; c < ESZ; ++c)
+                    *reinterpret_cast<uint4*>(slab + lane * 16 * ESZ + ((c ^ sw) << 4)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
                 fence_async_shared();
                 __syncwarp();
                 if (lane == 0) { tma_store_2d(&map_out, static_cast<int>(col0), tile_row0, slab); bulk_commit(); }
             } else if (row < g.M) {
                 TO* dst = static_cast<TO*>(g.out) + row * g.ldo + col0;
-                const uint32_t w[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
 #pragma unroll
-                for (int j = 0; j < 32 / ESZ; ++j)
+                for (int j = 0; j < 16; ++j)
                     if (col0 + j < g.N) {
-                        if constexpr (ESZ == 4) reinterpret_cast<uint32_t*>(dst)[j] = w[j & 7];
+                        if constexpr (ESZ == 4) reinterpret_cast<uint32_t*>(dst)[j] = w[j];
                         else reinterpret_cast<uint16_t*>(dst)[j] = static_cast<uint16_t>(w[j >> 1] >> ((j & 1) * 16));
                     }
             }
         };
-        for (int t = first_tile; t < total_tiles; t += tile_step, ++local) {
+        auto release = [&] {               // this warp has read what it reads of the shared columns
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) { if (leader) mbar_arrive(shared_drained); else mbar_arrive_leader(shared_drained); }
+        };
+        auto add_bias = [&](float (&v)[16], int64_t c0) {
+            if (!g.bias) return;
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (c0 + j < g.N) v[j] += bias_at(g, c0 + j);
+        };
+        bool ok = true;
+        for (int t = first_tile; t < total_tiles && ok; t += tile_step) {
             const int2 tile = tile_at(t, g.tiles_m, g.tiles_n);
             const int tm = tile.x * 2 + rank, tn = tile.y;
-            const int acc = local & 1;
-            if (!mbar_wait(&acc_full[acc], (local >> 1) & 1, abort_flag)) break;
-            tc_fence_after();
             const int tile_row0 = tm * 128 + sub * 32;
             const int64_t row = tile_row0 + lane, colbase = static_cast<int64_t>(tn) * 256;
-            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(sub * 32) << 16) + acc * ACC_STRIDE;
-            // unit i of this warp: the shared one first (the last two of stage 0, the first two of stage 1), then seven of its own
-            auto unit_of = [&](int i) { return i == 0 ? (acc == 0 ? 14 + half : half) : (acc == 0 ? 0 : 2) + half * 7 + (i - 1); };
-            auto read = [&](int i, uint32_t (&r)[16]) {
-                tc_ld16(taddr + unit_of(i) * 16, r);
-                tc_wait_ld();
-                if (i == 0) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) { if (leader) mbar_arrive(shared_drained); else mbar_arrive_leader(shared_drained); }
-                }
-                if (g.bias) {
-                    const int64_t c0 = colbase + unit_of(i) * 16;
-#pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        if (c0 + j < g.N) r[j] = __float_as_uint(__uint_as_float(r[j]) + bias_at(g, c0 + j));
-                }
-            };
+            const uint32_t lane_at = tmem_base + (static_cast<uint32_t>(sub * 32) << 16);
             if constexpr (ESZ == 2) {      // drain to packed registers, then store
-                uint32_t packed[64];
+                const int acc = local & 1;
+                if (!mbar_wait(&acc_full[acc], (local >> 1) & 1, abort_flag)) { ok = false; break; }
+                tc_fence_after();
+                // unit i of this warp: the shared one first (the last two of stage 0, the first two of stage 1), then seven of its own
+                auto unit_of = [&](int i) { return i == 0 ? (acc == 0 ? 14 + half : half) : (acc == 0 ? 0 : 2) + half * 7 + (i - 1); };
+                uint32_t packed[8][8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     uint32_t r[16];
-                    read(i, r);
+                    tc_ld16(lane_at + acc * ACC_STRIDE + unit_of(i) * 16, r);
+                    tc_wait_ld();
+                    if (i == 0) release();
+                    float v[16];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) packed[i * 8 + j] = pack2<TO>(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+                    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+                    add_bias(v, colbase + unit_of(i) * 16);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) packed[i][j] = pack2<TO>(v[2 * j], v[2 * j + 1]);
                 }
                 if (tile_row0 < g.M) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const int64_t col0 = colbase + unit_of(i) * 16;
-                        const uint32_t* q = packed + i * 8;
-                        if (col0 < g.N) emit(make_uint4(q[0], q[1], q[2], q[3]), make_uint4(q[4], q[5], q[6], q[7]), row, col0, tile_row0);
+                        if (col0 < g.N) emit(packed[i], row, col0, tile_row0);
                     }
                 }
-            } else {
-#pragma unroll 1
-                for (int i = 0; i < 8; ++i) {
-                    uint32_t r[16];
-                    read(i, r);
-                    const int64_t col0 = colbase + unit_of(i) * 16;
-                    if (tile_row0 < g.M && col0 < g.N) emit(make_uint4(r[0], r[1], r[2], r[3]), make_uint4(r[4], r[5], r[6], r[7]), row, col0, tile_row0);
-                    if (tile_row0 < g.M && col0 + 8 < g.N)
-                        emit(make_uint4(r[8], r[9], r[10], r[11]), make_uint4(r[12], r[13], r[14], r[15]), row, col0 + 8, tile_row0);
+                ++local;
+            } else {                       // eight units of its own throughout, summed over the chunks in registers
+                float sum[8][16];
+                for (int k0 = 0; k0 < g.k_tiles; k0 += CHUNK, ++local) {
+                    const int acc = local & 1;
+                    if (!mbar_wait(&acc_full[acc], (local >> 1) & 1, abort_flag)) { ok = false; break; }
+                    tc_fence_after();
+                    // the shared columns are the last two units of stage 0 (the upper half's) and the first two of stage 1 (the lower's)
+                    const bool holds_shared = half != acc;
+                    if (!holds_shared) release();
+                    auto drain = [&](auto rotated) {
+#pragma unroll
+                        for (int o = 0; o < 8; ++o) {
+                            const int u = decltype(rotated)::value ? (o + 6) & 7 : o;
+                            uint32_t r[16];
+                            tc_ld16(lane_at + acc * ACC_STRIDE + (half * 8 + u) * 16, r);
+                            tc_wait_ld();
+                            if (o == 1 && holds_shared) release();
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) sum[u][j] = k0 ? sum[u][j] + __uint_as_float(r[j]) : __uint_as_float(r[j]);
+                        }
+                    };
+                    if (half == 1 && acc == 0) drain(std::true_type{}); else drain(std::false_type{});
+                }
+                if (!ok) break;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int64_t col0 = colbase + (half * 8 + u) * 16;
+                    if (tile_row0 >= g.M || col0 >= g.N) continue;
+                    add_bias(sum[u], col0);
+                    uint32_t w[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(sum[u][j]);
+                    emit(w, row, col0, tile_row0);
                 }
             }
         }
@@ -302,9 +347,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 namespace split8 {
 constexpr int THREADS = 192, MAX_STAGES = 12;
 constexpr int SCALES = 2 * G8_SF;
-constexpr int SF_BASE = 128, SF_COLS = 8, TMEM_COLS = 256;
+constexpr int SF_COLS = 8;
 constexpr int PITCH = 132;                           // floats per row of the partial tile: lanes of a quarter warp hit different banks
-constexpr int BARS = 2 * MAX_STAGES + 1;
+constexpr int BARS = 2 * MAX_STAGES + 4;
 constexpr int FIXED = 1024 + 256;
 constexpr int SMEM = 6 * (2 * G8_OPERAND + SCALES) + FIXED;
 // Bytes in flight are what a few rows need (their k-tiles come from HBM at its latency): fewer rows of A, more stages.
@@ -335,8 +380,11 @@ fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     uint8_t* sf_smem = smem + depth * stage_operands;
     uint64_t* full = reinterpret_cast<uint64_t*>(sf_smem + depth * SCALES);
     uint64_t* empty = full + depth;
-    uint64_t* acc_full = empty + depth;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+    uint64_t* acc_full = empty + depth;           // two accumulators of 128 columns where the contraction goes in chunks, else one
+    uint64_t* acc_free = acc_full + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_free + 2);
+    constexpr bool CHUNKS = Chunked<TO>::value;
+    constexpr int SF_BASE = CHUNKS ? 256 : 128, TMEM_COLS = 2 * SF_BASE;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -346,7 +394,7 @@ fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     const int k0 = static_cast<int>(static_cast<int64_t>(g.k_tiles) * rank / splits), k1 = static_cast<int>(static_cast<int64_t>(g.k_tiles) * (rank + 1) / splits);
     if (threadIdx.x == 0) {
         for (int s = 0; s < depth; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        mbar_init(acc_full, 1);
+        for (int a = 0; a < 2; ++a) { mbar_init(&acc_full[a], 1); mbar_init(&acc_free[a], 4); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -391,36 +439,74 @@ fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         bool ok = true;
         int stage = 0;
         uint32_t phase = 0;
-        for (int i = 0; i < k1 - k0; ++i) {
-            if (!mbar_wait_warp(&full[stage], phase, abort_flag)) { ok = false; break; }
-            tc_fence_after();
-            if (elect_one()) {
-                const uint32_t sb = smem_u32(smem + stage * stage_operands), sa = sb + G8_OPERAND, sf = smem_u32(sf_smem + stage * SCALES);
-                const uint32_t tsfa = tmem_base + SF_BASE + (i & 1) * SF_COLS, tsfb = tsfa + 4;
-                tc_cp_sf(tsfa, scale_desc(sf + G8_SF));
-                tc_cp_sf(tsfb, scale_desc(sf));
-#pragma unroll
-                for (int kb = 0; kb < 4; ++kb)
-                    mma8<false>(tmem_base, operand_desc(sb + kb * 32), operand_desc(sa + kb * 32), idesc, (i | kb) ? 1u : 0u, tsfa, tsfb);
-                tc_commit(&empty[stage]);
+        for (int i0 = 0, i1, part = 0; i0 < k1 - k0 && ok; i0 = i1, ++part) {
+            i1 = CHUNKS ? min(i0 + CHUNK, k1 - k0) : k1 - k0;
+            const int acc = part & 1;
+            if (part > 1) {                     // this accumulator's last chunk has been read
+                if (!mbar_wait_warp(&acc_free[acc], ((part >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
+                tc_fence_after();
             }
-            __syncwarp();
-            if (++stage == depth) { stage = 0; phase ^= 1; }
-        }
-        if (ok && elect_one()) tc_commit(acc_full);
-        __syncwarp();
-    } else if (mbar_wait_warp(acc_full, 0, abort_flag)) {
-        // every MMA has read its operands: their shared memory takes the FP32 partial tile [rows of A][128]; a lane holds a
-        // column of it
-        tc_fence_after();
-        const uint32_t taddr = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-        float* mine = reinterpret_cast<float*>(smem) + (warp & 3) * 32 + lane;
-        for (int u = 0; u < g.a_rows; u += 16) {
-            uint32_t r[16];
-            tc_ld16(taddr + u, r);
-            tc_wait_ld();
+            for (int i = i0; i < i1; ++i) {
+                if (!mbar_wait_warp(&full[stage], phase, abort_flag)) { ok = false; break; }
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t sb = smem_u32(smem + stage * stage_operands), sa = sb + G8_OPERAND, sf = smem_u32(sf_smem + stage * SCALES);
+                    const uint32_t tsfa = tmem_base + SF_BASE + (i & 1) * SF_COLS, tsfb = tsfa + 4;
+                    tc_cp_sf(tsfa, scale_desc(sf + G8_SF));
+                    tc_cp_sf(tsfb, scale_desc(sf));
 #pragma unroll
-            for (int j = 0; j < 16; ++j) mine[(u + j) * PITCH] = __uint_as_float(r[j]);
+                    for (int kb = 0; kb < 4; ++kb)
+                        mma8<false>(tmem_base + acc * 128, operand_desc(sb + kb * 32), operand_desc(sa + kb * 32), idesc, (i > i0 || kb) ? 1u : 0u, tsfa, tsfb);
+                    tc_commit(&empty[stage]);
+                }
+                __syncwarp();
+                if (++stage == depth) { stage = 0; phase ^= 1; }
+            }
+            if (ok && elect_one()) tc_commit(&acc_full[acc]);
+            __syncwarp();
+        }
+    } else {
+        // Behind the last MMA every operand has been read: their shared memory takes the FP32 partial tile [rows of A][128]; a lane
+        // holds a column of it.
+        const uint32_t lane_at = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        float* mine = reinterpret_cast<float*>(smem) + (warp & 3) * 32 + lane;
+        if constexpr (CHUNKS) {
+            float sum[8][16];
+            bool ok = true;
+            for (int i0 = 0, part = 0; i0 < k1 - k0; i0 += CHUNK, ++part) {
+                const int acc = part & 1;
+                if (!mbar_wait_warp(&acc_full[acc], (part >> 1) & 1, abort_flag)) { ok = false; break; }
+                tc_fence_after();
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    if (u * 16 >= g.a_rows) continue;
+                    uint32_t r[16];
+                    tc_ld16(lane_at + acc * 128 + u * 16, r);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) sum[u][j] = part ? sum[u][j] + __uint_as_float(r[j]) : __uint_as_float(r[j]);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&acc_free[acc]);
+            }
+            if (ok) {
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    if (u * 16 >= g.a_rows) continue;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) mine[(u * 16 + j) * PITCH] = sum[u][j];
+                }
+            }
+        } else if (mbar_wait_warp(acc_full, 0, abort_flag)) {
+            tc_fence_after();
+            for (int u = 0; u < g.a_rows; u += 16) {
+                uint32_t r[16];
+                tc_ld16(lane_at + u, r);
+                tc_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) mine[(u + j) * PITCH] = __uint_as_float(r[j]);
+            }
         }
     }
     tc_fence_before();
@@ -563,8 +649,8 @@ static int launch_gemm8(Gemm8Args& g, const uint8_t* a, const CUtensorMap& mb, c
         CUtensorMap mo = ma;           // unused without tma_store, but the parameter must hold a valid map
         constexpr int ESZ = sizeof(TO);
         g.tma_store = aligned(g.out, 16) && g.ldo * ESZ % 16 == 0 &&
-                      map_2d(&mo, ESZ == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, g.out, g.N, g.M, g.ldo * ESZ, 32 / ESZ, 32,
-                             CU_TENSOR_MAP_SWIZZLE_32B);
+                      map_2d(&mo, ESZ == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, g.out, g.N, g.M, g.ldo * ESZ, 16, 32,
+                             ESZ == 4 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
         attr[0].val.clusterDim.x = 2;
         cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min<int64_t>(static_cast<int64_t>(g.tiles_m) * g.tiles_n, slots[dev].pairs)));
         cfg.blockDim = dim3(pair8::THREADS);
