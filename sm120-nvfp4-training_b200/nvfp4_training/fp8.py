@@ -16,7 +16,7 @@ import torch
 from torch import nn
 
 from . import _native as nat
-from .operators import _check_device, _check_tensor, _once, pitch_of, rows_of
+from .operators import _autograd_sees, _check_device, _check_tensor, _once, pitch_of, rows_of
 
 _MAX = 1 << 30
 
@@ -192,7 +192,7 @@ def fp8_linear(x, weight, bias=None):
     _check_device(x)
     if packed is not None:
         weight = None
-    if not (torch.is_grad_enabled() and (x.requires_grad or any(t is not None and t.requires_grad for t in (weight, bias)))):
+    if not _autograd_sees(x, weight, bias):
         return _forward(x, weight, bias, packed, False, False)[0]
     return _Fp8Linear.apply(x, weight, bias, packed)
 

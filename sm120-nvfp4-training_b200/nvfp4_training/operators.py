@@ -1,6 +1,6 @@
 """Operators of an image / video transformer block: layer norm with the residual sum in front of it, and rotary positions over
 several axes.  The kernels are nvfp4_layer_norm / nvfp4_layer_norm_bwd and nvfp4_rotary_axes of the C-ABI library; everything
-here is differentiable once and may be captured into a CUDA graph.
+here is differentiable once (in backward mode; forward-mode tangents are refused) and may be captured into a CUDA graph.
 """
 from __future__ import annotations
 
@@ -11,6 +11,7 @@ from functools import lru_cache
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 
 from . import _native as nat
 from ._backend.quant import attach_amax
@@ -29,6 +30,13 @@ def _check_device(t):
     """Last of an operator's checks: the arguments fit together, now they also have to be on a GPU."""
     if not t.is_cuda:
         raise ValueError("This operator needs CUDA tensors")
+
+
+def _autograd_sees(*tensors):
+    """Whether a call has to go through its autograd.Function: a gradient may be asked for, or a forward-mode level is open, whose
+    tangents only the Function can refuse (a dual tensor has no requires_grad, and a result made without it would count as
+    constant)."""
+    return forward_ad._current_level >= 0 or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
 
 
 def _zeroed_slot(device):
@@ -173,7 +181,7 @@ def _layer_norm(x, delta, weight, bias, eps, out_dtype, want_amax=False):
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError("weight and bias must have one dtype")
     _check_device(x)
-    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, delta, weight, bias))):
+    if not _autograd_sees(x, delta, weight, bias):
         amax = _zeroed_slot(x.device) if want_amax and out_dtype == torch.bfloat16 else None
         total, h, _ = _norm_forward(x, delta, weight, bias, eps, out_dtype, amax, False)
         return (None if delta is None else total if x.ndim == 2 else total.view(x.shape)), h, amax
@@ -350,7 +358,7 @@ def rotary_axes(q, k, positions, sections, *, theta=10000.0, layout="half", freq
     if q.shape[2] == 0:
         raise ValueError("q needs at least one head")
     how = _check_rotary(q, q.shape[0], q.shape[1], q.shape[3], positions, sections, theta, layout, frequencies)
-    if not (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
+    if not _autograd_sees(q, k):
         return tuple(_turn((q, k), positions, how, False))
     return _RotaryAxes.apply(q, k, positions, how)
 
@@ -367,7 +375,7 @@ def rotary_axes_qkv(qkv, positions, sections, heads, kv_heads=None, *, theta=100
     dim = qkv.shape[2] // (heads + 2 * kv_heads)
     how = _check_rotary(qkv, qkv.shape[0], qkv.shape[1], dim, positions, sections, theta, layout, frequencies)
     qkv = _features_contiguous(qkv)
-    if not (torch.is_grad_enabled() and qkv.requires_grad):
+    if not _autograd_sees(qkv):
         q, k, v = _split_heads(qkv, heads, kv_heads)
         return (*_turn((q, k), positions, how, False), v)
     return _RotaryFused.apply(qkv, positions, how, heads, kv_heads)

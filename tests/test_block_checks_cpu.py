@@ -1,0 +1,56 @@
+"""Calls of the transformer-block operators that need no GPU to be seen: the kernels are replaced by formulas here, so that what
+the public functions hand to autograd, to the optimizer and to other ranks can be held against what they should."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import nvfp4_training as nv
+from nvfp4_training import fp8, operators
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+@pytest.fixture
+def without_kernels(monkeypatch):
+    """The operators' host side on CPU tensors, with results that depend on nothing but shapes."""
+    for module in (operators, fp8):
+        monkeypatch.setattr(module, "_check_device", lambda t: None)
+
+    def norm(x, delta, weight, bias, eps, out_dtype, amax, keep_stats):
+        rows = x.reshape(-1, x.shape[-1])
+        return rows if delta is None else rows * 1, x.to(out_dtype) * 1, torch.zeros(2 * len(rows)) if keep_stats else None
+    monkeypatch.setattr(operators, "_norm_forward", norm)
+    monkeypatch.setattr(operators, "_turn", lambda tensors, positions, how, inverse: [None if t is None else t * 1 for t in tensors])
+    monkeypatch.setattr(fp8, "_forward", lambda x, weight, bias, packed, need_x, need_w: (x.new_zeros(*x.shape[:-1], weight.shape[0]), None, None))
+
+
+T, W, POS = torch.ones(2, 3, 12), torch.ones(12), torch.zeros(3, 1, dtype=torch.float64)
+Q = torch.ones(2, 3, 4, 4)
+CALLS = {
+    "layer_norm x": (lambda t: nv.layer_norm(t, W), T),
+    "layer_norm weight": (lambda t: nv.layer_norm(T, t), W),
+    "layer_norm bias": (lambda t: nv.layer_norm(T, None, t), W),
+    "add_layer_norm x": (lambda t: nv.add_layer_norm(t, T), T),
+    "add_layer_norm delta": (lambda t: nv.add_layer_norm(T, t), T),
+    "LayerNorm": (lambda t: nv.LayerNorm(12)(t), T),
+    "rotary_axes q": (lambda t: nv.rotary_axes(t, Q, POS, (2,)), Q),
+    "rotary_axes k": (lambda t: nv.rotary_axes(Q, t, POS, (2,)), Q),
+    "rotary_axes positions": (lambda t: nv.rotary_axes(Q, None, t, (2,)), POS),
+    "rotary_axes_qkv": (lambda t: nv.rotary_axes_qkv(t, POS, (2,), 1), T),
+    "fp8_linear x": (lambda t: nv.fp8_linear(t, torch.ones(5, 12)), T),
+    "fp8_linear weight": (lambda t: nv.fp8_linear(T, t), torch.ones(5, 12)),
+    "fp8_linear bias": (lambda t: nv.fp8_linear(T, torch.ones(5, 12), t), torch.ones(5)),
+}
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("name", CALLS)
+def test_forward_mode_tangents_are_refused(without_kernels, name, grad):
+    """A tangent that an operator cannot carry on is an error, never a result that passes for constant."""
+    call, at = CALLS[name]
+    with torch.set_grad_enabled(grad):
+        call(at)                                                   # no level is open
+        with forward_ad.dual_level():
+            call(at)                                               # no tangent
+            with pytest.raises(NotImplementedError):
+                call(forward_ad.make_dual(at, torch.ones_like(at)))
