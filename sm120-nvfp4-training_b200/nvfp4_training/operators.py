@@ -207,7 +207,15 @@ class LayerNorm(nn.LayerNorm):
     """nn.LayerNorm over the last dimension on this library's kernels (same parameters and state dict).  Under CUDA BF16
     autocast an FP32 input gives a BF16 result, which is what the next converted layer reads; BF16 results carry their amax."""
 
+    def __init__(self, normalized_shape, *args, **options):
+        super().__init__(normalized_shape, *args, **options)
+        if len(self.normalized_shape) != 1:
+            raise ValueError("LayerNorm works over the last dimension alone; nn.LayerNorm takes several")
+
     def forward(self, x):
+        # without affine parameters nothing else holds x against the shape that the module was made for
+        if not isinstance(x, torch.Tensor) or x.shape[-1:] != tuple(self.normalized_shape):
+            raise ValueError(f"x must have a last dimension of {tuple(self.normalized_shape)}")
         out = torch.bfloat16 if (x.dtype == torch.float32 and torch.is_autocast_enabled("cuda")
                                  and torch.get_autocast_dtype("cuda") == torch.bfloat16) else x.dtype
         _, h, amax = _layer_norm(x, None, self.weight, self.bias, self.eps, out, want_amax=True)

@@ -54,3 +54,19 @@ def test_forward_mode_tangents_are_refused(without_kernels, name, grad):
             call(at)                                               # no tangent
             with pytest.raises(NotImplementedError):
                 call(forward_ad.make_dual(at, torch.ones_like(at)))
+
+
+@pytest.mark.parametrize("affine", [True, False])
+def test_layer_norm_module_holds_its_shape(without_kernels, affine):
+    make = lambda shape: nv.LayerNorm(shape, elementwise_affine=affine)
+    assert make(8)(torch.ones(2, 8)).shape == (2, 8) and make((8,))(torch.ones(8)).shape == (8,)
+    for x in (torch.ones(2, 16), torch.ones(8, 2), torch.ones(()), torch.ones(2, 0)):
+        with pytest.raises(ValueError):
+            make(8)(x)
+    for shape in ((3, 16), ()):
+        with pytest.raises(ValueError):
+            make(shape)
+    swapped = torch.nn.LayerNorm((3, 16), elementwise_affine=affine)          # a module made by nn.LayerNorm, then given this class
+    swapped.__class__ = nv.LayerNorm
+    with pytest.raises(ValueError):
+        swapped(torch.ones(3, 16))
