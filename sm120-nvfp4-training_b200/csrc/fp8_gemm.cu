@@ -2,8 +2,8 @@
 //
 // tcgen05.mma.kind::mxf8f6f4 multiplies a UE8M0 scale into every 32 elements of the contraction; the packings give the four
 // 32-blocks of a 128-block the same byte, so the tensor cores apply the block scale themselves and accumulate in FP32 tensor
-// memory, over the whole contraction for a 16-bit result (CHUNK below has the rule for FP32 ones), without a pass of
-// multiply-adds per block on the CUDA cores.
+// memory, emptied into registers only where a long contraction would lose bits there (CHUNK below), without a pass of multiply-adds
+// per block on the CUDA cores.
 //
 // Two kernels.
 //   fp8_gemm_kernel        persistent clusters of two CTAs on 256 x 256 tiles (cta_group::2, M256 x N256 x K32 instructions), for
@@ -32,15 +32,17 @@ constexpr int G8_BK = 128;                  // elements (and bytes) of the contr
 constexpr int G8_SF = 512;                  // bytes of a scale block: 128 rows x 4
 constexpr int G8_OPERAND = 128 * 128;       // bytes of 128 rows of an operand per stage
 
-// The tensor cores drop bits towards zero when they add to an accumulator, so a sum of terms of one sign falls behind steadily
-// (measured relative error of the paired kernel, positive operands: 5e-7 after 2048 elements, 1.4e-6 after 4096, 9.9e-6 after
-// 16384, 1.05e-4 after 66000; signs that cancel: 1.1e-7, 2.2e-7, 1.2e-6 after 16384).  A 16-bit result is itself rounded by 2e-3
-// (BF16) or 5e-4 (FP16) and keeps the one accumulator.  For FP32 results
-// the accumulator is emptied into FP32 registers every CHUNK k-tiles (2048 elements): 5e-7 (1.2e-7) whatever the length.  Between
-// chunks the tensor cores wait about 0.6 us for the epilogue: 14336 x 4096 x 8192 341 -> 364 us, 8192 x 4096 x 4096 100 -> 106;
-// up to 2048 elements nothing.  Chunks of 1024 bring 1.9e-7 and cost 14 to 20 %; of 4096, 1.4e-6 and 4 to 5 %.
-constexpr int CHUNK = 16;
-template <typename TO> struct Chunked { static constexpr bool value = sizeof(TO) == 4; };
+// The tensor cores drop bits towards zero when they add to an accumulator, so a sum of terms of one sign falls behind steadily,
+// and faster the longer it is (measured relative error of the paired kernel, positive operands: 5e-7 after 2048 elements, 1.4e-6
+// after 4096, 9.9e-6 after 16384, 1.05e-4 after 66000; signs that cancel: 1.1e-7, 2.2e-7, 1.2e-6 after 16384).  So a contraction
+// goes in chunks of CHUNK k-tiles, between which the accumulator is emptied into FP32 registers, and the error is that of one chunk
+// whatever the length.  FP32 results: 2048 elements, 5e-7 (1.2e-7).  The tensor cores wait about 0.6 us for the epilogue between
+// chunks: 14336 x 4096 x 8192 341 -> 364 us, 8192 x 4096 x 4096 100 -> 106; chunks of 1024 bring 1.9e-7 and cost 14 to 20 %; of
+// 4096, 1.4e-6 and 4 to 5 %.  16-bit results are rounded by half a step of 3.9e-3 (BF16) or 4.9e-4 (FP16) and take 4096 elements,
+// 1.4e-6; up to there they keep the one accumulator and packed registers of a kernel without chunks.  Against no chunks,
+// 14336 x 4096 x 16384 BF16 comes to the other neighbour of the exact sum in 0.035 % of the elements instead of 0.12 % (a sum in
+// FP32: 0.02 %), and 16384 x 4096 x 14336 takes 705 instead of 682 us; chunks of 8192: 0.07 % and 698 us.
+template <typename TO> constexpr int CHUNK = sizeof(TO) == 4 ? 16 : 32;
 
 struct Gemm8Args {
     const void* bias;
@@ -103,7 +105,7 @@ constexpr int SMEM = STAGES * STAGE_BYTES + EPI_WARPS * STAGING + 1024 + 256;
 static_assert(SF_BASE + 2 * SF_COLS <= TMEM_COLS && BARS * 8 + 16 <= 256 && SMEM <= 232448, "budgets");
 }  // namespace pair8
 
-template <typename TO>
+template <typename TO, bool CHUNKS>
 __global__ void __launch_bounds__(pair8::THREADS, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_sfa,
                 const __grid_constant__ CUtensorMap map_sfb, const __grid_constant__ CUtensorMap map_out, const Gemm8Args g) {
@@ -186,7 +188,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             bool ok = true;
             for (int t = first_tile; t < total_tiles && ok; t += tile_step) {
                 for (int k0 = 0, k1; k0 < g.k_tiles && ok; k0 = k1, ++local) {       // a chunk, or the whole contraction
-                    k1 = Chunked<TO>::value ? min(k0 + CHUNK, g.k_tiles) : g.k_tiles;
+                    k1 = CHUNKS ? min(k0 + CHUNK<TO>, g.k_tiles) : g.k_tiles;
                     const int acc = local & 1;
                     const uint32_t tmem_acc = tmem_base + acc * ACC_STRIDE;
                     if (local > 0) {       // the shared columns of the one before are read, and with them everything of the one before that
@@ -265,7 +267,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             const int tile_row0 = tm * 128 + sub * 32;
             const int64_t row = tile_row0 + lane, colbase = static_cast<int64_t>(tn) * 256;
             const uint32_t lane_at = tmem_base + (static_cast<uint32_t>(sub * 32) << 16);
-            if constexpr (ESZ == 2) {      // drain to packed registers, then store
+            if constexpr (!CHUNKS) {       // drain to packed registers, then store
                 const int acc = local & 1;
                 if (!mbar_wait(&acc_full[acc], (local >> 1) & 1, abort_flag)) { ok = false; break; }
                 tc_fence_after();
@@ -293,9 +295,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                     }
                 }
                 ++local;
-            } else {                       // eight units of its own throughout, summed over the chunks in registers
+            } else {                       // eight units of its own throughout, summed over the chunks in registers, rounded once
                 float sum[8][16];
-                for (int k0 = 0; k0 < g.k_tiles; k0 += CHUNK, ++local) {
+                for (int k0 = 0; k0 < g.k_tiles; k0 += CHUNK<TO>, ++local) {
                     const int acc = local & 1;
                     if (!mbar_wait(&acc_full[acc], (local >> 1) & 1, abort_flag)) { ok = false; break; }
                     tc_fence_after();
@@ -322,9 +324,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                     const int64_t col0 = colbase + (half * 8 + u) * 16;
                     if (tile_row0 >= g.M || col0 >= g.N) continue;
                     add_bias(sum[u], col0);
-                    uint32_t w[16];
+                    uint32_t w[4 * ESZ];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(sum[u][j]);
+                    for (int j = 0; j < 4 * ESZ; ++j) {
+                        if constexpr (ESZ == 2) w[j] = pack2<TO>(sum[u][2 * j], sum[u][2 * j + 1]);
+                        else w[j] = __float_as_uint(sum[u][j]);
+                    }
                     emit(w, row, col0, tile_row0);
                 }
             }
@@ -369,7 +374,7 @@ __device__ __forceinline__ float4 cluster_load4(uint32_t addr, int rank) {     /
     return v;
 }
 
-template <typename TO>
+template <typename TO, bool CHUNKS>
 __global__ void __launch_bounds__(split8::THREADS, 1)
 fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_sfa,
                       const __grid_constant__ CUtensorMap map_sfb, const Gemm8Args g, const int splits) {
@@ -383,7 +388,6 @@ fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     uint64_t* acc_full = empty + depth;           // two accumulators of 128 columns where the contraction goes in chunks, else one
     uint64_t* acc_free = acc_full + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_free + 2);
-    constexpr bool CHUNKS = Chunked<TO>::value;
     constexpr int SF_BASE = CHUNKS ? 256 : 128, TMEM_COLS = 2 * SF_BASE;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -440,7 +444,7 @@ fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         int stage = 0;
         uint32_t phase = 0;
         for (int i0 = 0, i1, part = 0; i0 < k1 - k0 && ok; i0 = i1, ++part) {
-            i1 = CHUNKS ? min(i0 + CHUNK, k1 - k0) : k1 - k0;
+            i1 = CHUNKS ? min(i0 + CHUNK<TO>, k1 - k0) : k1 - k0;
             const int acc = part & 1;
             if (part > 1) {                     // this accumulator's last chunk has been read
                 if (!mbar_wait_warp(&acc_free[acc], ((part >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
@@ -473,7 +477,7 @@ fp8_gemm_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         if constexpr (CHUNKS) {
             float sum[8][16];
             bool ok = true;
-            for (int i0 = 0, part = 0; i0 < k1 - k0; i0 += CHUNK, ++part) {
+            for (int i0 = 0, part = 0; i0 < k1 - k0; i0 += CHUNK<TO>, ++part) {
                 const int acc = part & 1;
                 if (!mbar_wait_warp(&acc_full[acc], (part >> 1) & 1, abort_flag)) { ok = false; break; }
                 tc_fence_after();
@@ -598,7 +602,7 @@ static int split_for(const Gemm8Args& g, const Slots& slots) {
     return pick;
 }
 
-template <typename TO>
+template <typename TO, bool CHUNKS>
 static int launch_gemm8(Gemm8Args& g, const uint8_t* a, const CUtensorMap& mb, const CUtensorMap& msa, const CUtensorMap& msb, cudaStream_t st) {
     int dev = 0;
     cudaGetDevice(&dev);
@@ -606,8 +610,8 @@ static int launch_gemm8(Gemm8Args& g, const uint8_t* a, const CUtensorMap& mb, c
     static Slots slots[64] = {};
     NVFP4_REQUIRE(dev >= 0 && dev < 64, NVFP4_ERR_UNSUPPORTED, "nvfp4_fp8_gemm: device index above 63");
     if (!configured[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(fp8_gemm_kernel<TO>, cudaFuncAttributeMaxDynamicSharedMemorySize, pair8::SMEM);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_gemm_split_kernel<TO>, cudaFuncAttributeMaxDynamicSharedMemorySize, split8::SMEM);
+        cudaError_t e = cudaFuncSetAttribute(fp8_gemm_kernel<TO, CHUNKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, pair8::SMEM);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_gemm_split_kernel<TO, CHUNKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, split8::SMEM);
         // clusters do not fill every SM (a group of SMs holds whole clusters only): what the device says it runs at once
         cudaLaunchConfig_t c = {};
         cudaLaunchAttribute size[1];
@@ -620,13 +624,13 @@ static int launch_gemm8(Gemm8Args& g, const uint8_t* a, const CUtensorMap& mb, c
             c.gridDim = dim3(8);
             c.blockDim = dim3(split8::THREADS);
             c.dynamicSmemBytes = split8::SMEM;
-            e = cudaOccupancyMaxActiveClusters(&slots[dev].clusters[i], fp8_gemm_split_kernel<TO>, &c);
+            e = cudaOccupancyMaxActiveClusters(&slots[dev].clusters[i], fp8_gemm_split_kernel<TO, CHUNKS>, &c);
         }
         if (e == cudaSuccess) {
             size[0].val.clusterDim.x = 2;
             c.blockDim = dim3(pair8::THREADS);
             c.dynamicSmemBytes = pair8::SMEM;
-            e = cudaOccupancyMaxActiveClusters(&slots[dev].pairs, fp8_gemm_kernel<TO>, &c);
+            e = cudaOccupancyMaxActiveClusters(&slots[dev].pairs, fp8_gemm_kernel<TO, CHUNKS>, &c);
         }
         NVFP4_REQUIRE(e == cudaSuccess && slots[dev].pairs > 0, NVFP4_ERR_LAUNCH, "nvfp4_fp8_gemm: cannot configure the kernels: %s", cudaGetErrorString(e));
         configured[dev] = true;
@@ -655,7 +659,7 @@ static int launch_gemm8(Gemm8Args& g, const uint8_t* a, const CUtensorMap& mb, c
         cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min<int64_t>(static_cast<int64_t>(g.tiles_m) * g.tiles_n, slots[dev].pairs)));
         cfg.blockDim = dim3(pair8::THREADS);
         cfg.dynamicSmemBytes = pair8::SMEM;
-        e = cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<TO>, ma, mb, msa, msb, mo, g);
+        e = cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<TO, CHUNKS>, ma, mb, msa, msb, mo, g);
     } else {
         g.tiles_m = (g.M + 127) / 128;
         g.tiles_n = (g.N + 127) / 128;
@@ -663,7 +667,7 @@ static int launch_gemm8(Gemm8Args& g, const uint8_t* a, const CUtensorMap& mb, c
         cfg.gridDim = dim3(static_cast<unsigned>(g.tiles_m * g.tiles_n * splits));
         cfg.blockDim = dim3(split8::THREADS);
         cfg.dynamicSmemBytes = split8::SMEM;
-        e = cudaLaunchKernelEx(&cfg, fp8_gemm_split_kernel<TO>, ma, mb, msa, msb, g, splits);
+        e = cudaLaunchKernelEx(&cfg, fp8_gemm_split_kernel<TO, CHUNKS>, ma, mb, msa, msb, g, splits);
     }
     NVFP4_REQUIRE(e == cudaSuccess, NVFP4_ERR_LAUNCH, "nvfp4_fp8_gemm: cluster launch failed: %s", cudaGetErrorString(e));
     return launch_status("nvfp4_fp8_gemm");
@@ -694,9 +698,10 @@ extern "C" int nvfp4_fp8_gemm(const uint8_t* a, const uint8_t* a_scales, const u
     NVFP4_REQUIRE(operand_map(&mb, b, N, K, 128) && scale_map(&msa, a_scales, M, K) && scale_map(&msb, b_scales, N, K),
                   NVFP4_ERR_LAUNCH, "nvfp4_fp8_gemm: cuTensorMapEncodeTiled failed or is unavailable");
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (out_dtype == NVFP4_BF16) return launch_gemm8<__nv_bfloat16>(g, a, mb, msa, msb, st);
-    if (out_dtype == NVFP4_F16) return launch_gemm8<__half>(g, a, mb, msa, msb, st);
-    return launch_gemm8<float>(g, a, mb, msa, msb, st);
+    const bool chunks = g.k_tiles > CHUNK<__half>;
+    if (out_dtype == NVFP4_BF16) return chunks ? launch_gemm8<__nv_bfloat16, true>(g, a, mb, msa, msb, st) : launch_gemm8<__nv_bfloat16, false>(g, a, mb, msa, msb, st);
+    if (out_dtype == NVFP4_F16) return chunks ? launch_gemm8<__half, true>(g, a, mb, msa, msb, st) : launch_gemm8<__half, false>(g, a, mb, msa, msb, st);
+    return launch_gemm8<float, true>(g, a, mb, msa, msb, st);
 }
 
 extern "C" int64_t nvfp4_fp8_packing_bytes(int64_t rows, int64_t k) {
