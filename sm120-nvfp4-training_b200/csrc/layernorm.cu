@@ -5,7 +5,8 @@
 //
 // Both directions stream: every operand is read once and every result written once, so HBM is the bound.  A row stays in
 // registers between the sweeps over it (sum, centred squares, result); squares are taken around a mean, never as a difference of
-// sums, which keeps the variance exact where the mean is large against the spread.  All statistics are FP32; a result is
+// sums, which keeps the variance exact where the mean is large against the spread, and means are rounded once (Reciprocal
+// below): a constant row whose sum FP32 holds gives differences of exactly zero.  All statistics are FP32; a result is
 // rounded once, except that h is formed from the total as it is stored (the backward pass reads that one too).  Rows that
 // bulk copies can fetch go through the ring further down (16384 x 5120 BF16 with the residual sum: forward 109 us, 0.95 of the
 // measured HBM rate, backward 137 us, 0.76); the kernels before it take the odd widths, the unaligned rows and the widest.
@@ -36,6 +37,15 @@ __device__ __forceinline__ float cta_sum(float v, float* slots) {
     __syncthreads();
     return warp_sum(lane < warps ? slots[lane] : 0.f);
 }
+
+// 1 / n in two parts, so that a sum's mean is off by 2^-46 before its one rounding: where the quotient is a float, as for constant
+// rows, it is that float.  (One product more than with a rounded 1 / n; a division for each mean took 122 instead of 106 us for
+// 16384 x 5120 BF16, 22.6 instead of 13.9 for 32768 x 256.)
+struct Reciprocal {
+    float high, low;
+    __device__ __forceinline__ explicit Reciprocal(float n) : high(1.f / n), low(fmaf(-high, n, 1.f) * high) {}
+    __device__ __forceinline__ float of(float sum) const { return fmaf(sum, high, sum * low); }
+};
 
 // V elements of total at column c of row r (stored, too, when there is a delta), as FP32
 template <typename TX, int V>
@@ -81,7 +91,7 @@ __global__ void __launch_bounds__(ROW_CTA ? 1024 : 256) norm_fwd_kernel(const No
     const int64_t row0 = ROW_CTA ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
     const int64_t row_step = ROW_CTA ? gridDim.x : static_cast<int64_t>(gridDim.x) * 8;
     const int vectors = a.cols / V;
-    const float inv_n = 1.f / static_cast<float>(a.cols);
+    const Reciprocal inv_n(static_cast<float>(a.cols));
     float best = 0.f;
     for (int64_t r = row0; r < a.rows; r += row_step) {
         float f[N][V];
@@ -95,7 +105,7 @@ __global__ void __launch_bounds__(ROW_CTA ? 1024 : 256) norm_fwd_kernel(const No
                 for (int j = 0; j < V; ++j) s += f[i][j];
             }
         }
-        const float mean = (ROW_CTA ? cta_sum(s, slots[0]) : warp_sum(s)) * inv_n;
+        const float mean = inv_n.of(ROW_CTA ? cta_sum(s, slots[0]) : warp_sum(s));
         float sq = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -103,7 +113,7 @@ __global__ void __launch_bounds__(ROW_CTA ? 1024 : 256) norm_fwd_kernel(const No
 #pragma unroll
                 for (int j = 0; j < V; ++j) { const float d = f[i][j] - mean; sq = fmaf(d, d, sq); }
             }
-        const float rstd = rsqrtf((ROW_CTA ? cta_sum(sq, slots[1]) : warp_sum(sq)) * inv_n + a.eps);
+        const float rstd = rsqrtf((ROW_CTA ? cta_sum(sq, slots[1]) : warp_sum(sq)) * inv_n.high + a.eps);
         if (tid == 0 && a.mean) { a.mean[r] = mean; a.rstd[r] = rstd; }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -545,9 +555,9 @@ __global__ void __launch_bounds__(MAXT, CTAS) norm_fwd_ring_kernel(const NormArg
     if (lane == 0) slots[0][0][threadIdx.x >> 5].x = mine;
     __syncthreads();
     const float theirs = lane < warps ? slots[0][0][first_warp + lane].x : 0.f;
-    const float inv_mine = mine > 0.f ? 1.f / mine : 0.f, inv_theirs = theirs > 0.f ? 1.f / theirs : 0.f;
+    // (a warp without columns has sums of zero)
+    const Reciprocal inv_mine(fmaxf(mine, 1.f)), inv_theirs(fmaxf(theirs, 1.f)), inv_n(static_cast<float>(a.cols));
     int half = 1;
-    const float inv_n = 1.f / static_cast<float>(a.cols);
     float best = 0.f;
     for (int64_t g = blockIdx.x; g < runs; g += gridDim.x, half ^= 1) {
         aop::mbar_wait(&q.full[at.slot], at.phase, &q.abort_flag);
@@ -581,7 +591,7 @@ __global__ void __launch_bounds__(MAXT, CTAS) norm_fwd_ring_kernel(const NormArg
         for (int k = 0; k < R; ++k) sums[k] = warp_sum(sums[k]);
 #pragma unroll
         for (int k = 0; k < R; ++k) {
-            const float m = sums[k] * inv_mine;
+            const float m = inv_mine.of(sums[k]);
             squares[k] = 0.f;
 #pragma unroll
             for (int i = 0; i < N; ++i)
@@ -606,17 +616,19 @@ __global__ void __launch_bounds__(MAXT, CTAS) norm_fwd_ring_kernel(const NormArg
             }
 #pragma unroll
             for (int k = 0; k < R; ++k) {
-                const float d = part[k].x * inv_theirs - sums[k] * inv_n;
+                mean[k] = inv_n.of(sums[k]);
+                const float d = inv_theirs.of(part[k].x) - mean[k];
                 squares[k] = warp_sum(fmaf(theirs * d, d, part[k].y));
             }
-        }
+        } else {
 #pragma unroll
-        for (int k = 0; k < R; ++k) mean[k] = sums[k] * inv_n;
+            for (int k = 0; k < R; ++k) mean[k] = inv_n.of(sums[k]);
+        }
 #pragma unroll
         for (int k = 0; k < R; ++k) {
             const int64_t r = g * per_stage + group * R + k;
             if (r >= a.rows) continue;
-            const float rstd = rsqrtf(squares[k] * inv_n + a.eps);
+            const float rstd = rsqrtf(squares[k] * inv_n.high + a.eps);
             if (tid == 0 && a.mean) { a.mean[r] = mean[k]; a.rstd[r] = rstd; }
 #pragma unroll
             for (int i = 0; i < N; ++i) {
