@@ -8,8 +8,8 @@
 // sums, which keeps the variance exact where the mean is large against the spread, and means are rounded once (Reciprocal
 // below): a constant row whose sum FP32 holds gives differences of exactly zero.  All statistics are FP32; a result is
 // rounded once, except that h is formed from the total as it is stored (the backward pass reads that one too).  Rows that
-// bulk copies can fetch go through the ring further down (16384 x 5120 BF16 with the residual sum: forward 109 us, 0.95 of the
-// measured HBM rate, backward 137 us, 0.76); the kernels before it take the odd widths, the unaligned rows and the widest.
+// bulk copies can fetch go through the ring further down (16384 x 5120 BF16 with the residual sum: forward 106 us, 0.98 of the
+// measured HBM rate, backward 142 us, 0.73); the kernels before it take the odd widths, the unaligned rows and the widest.
 #include "async.cuh"
 #include "bf16x8.cuh"
 #include "vec.cuh"
@@ -709,7 +709,6 @@ __global__ void __launch_bounds__(MAXT, CTAS) norm_bwd_ring_kernel(const NormBwd
 #pragma unroll
         for (int k = 0; k < R; ++k) {
             rs[k] = rstd[k];
-            const float shift = -mean[k] * rstd[k];
             sums[2 * k] = sums[2 * k + 1] = 0.f;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -728,7 +727,7 @@ __global__ void __launch_bounds__(MAXT, CTAS) norm_bwd_ring_kernel(const NormBwd
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const float dh = u[k][i][j];
-                    z[k][i][j] = fmaf(z[k][i][j], rs[k], shift);
+                    z[k][i][j] = (z[k][i][j] - mean[k]) * rs[k];      // not x rstd - mean rstd, whose rounding is large where the mean is
                     acc_w[i][j] = fmaf(dh, z[k][i][j], acc_w[i][j]);
                     acc_b[i][j] += dh;
                     u[k][i][j] = dh * w[i][j];

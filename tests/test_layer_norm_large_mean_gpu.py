@@ -33,3 +33,18 @@ def test_constant_rows_give_the_bias(cols, dtype, out_dtype):
     assert torch.equal(nv.layer_norm(x, w, b, out_dtype=out_dtype), want)
     total, h = nv.add_layer_norm(x, torch.zeros_like(x), w, b, out_dtype=out_dtype)
     assert torch.equal(h, want) and torch.equal(total, x)
+
+
+@widths
+@types
+def test_constant_rows_leave_the_weight_alone(cols, dtype, out_dtype):
+    x, w, b, dh = constant_rows(cols, dtype, out_dtype)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(nv.layer_norm(*leaves, out_dtype=out_dtype), leaves, dh)
+    assert not dw.any()
+    u = dh.double() * w.double()
+    want = (u - u.mean(-1, keepdim=True)) * 1e-5 ** -0.5
+    # a product, a mean over a tree of sums, two more operations and rsqrt in FP32, each below 2^-22 of the largest |u| rstd
+    bound = torch.finfo(dtype).eps / 2 * 1.01 * want.abs() + 2.0 ** -18 * u.abs().max(-1, keepdim=True).values * 1e-5 ** -0.5
+    assert bool(((dx.double() - want).abs() <= bound).all())
+    assert bool(((db.double() - dh.double().sum(0)).abs() <= 2.0 ** -21 * dh.double().abs().sum(0)).all())
