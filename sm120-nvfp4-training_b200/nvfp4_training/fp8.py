@@ -117,17 +117,20 @@ class _Fp8Linear(torch.autograd.Function):
         dev = grad.device
         dx = grad.new_empty(shape, dtype=dtype) if need_x else None
         db = None if b_dtype is None else grad.new_empty(n, dtype=b_dtype)
-        if not m:
-            return dx, (torch.zeros(weight.shape, dtype=weight.dtype, device=dev) if need_w else None), (None if db is None else db.zero_()), None
         dw, taken = _weight_gradient_into(weight) if need_w else (None, None)
-        columns = need_w or db is not None
-        work = _bytes((_packing_bytes(m, n) if need_x else 0) + (_packing_bytes(n, m) + 4 * n * _ceil128(m) if columns else 0), grad)
-        g = rows_of(grad, n)
-        codes = nat._CODES
-        with nat.on(dev):
-            nat.check(nat.lib().nvfp4_fp8_linear_bwd(g.data_ptr(), codes[g.dtype], m, n, k, pitch_of(g), nat.ptr(x_t), nat.ptr(w_t), nat.ptr(dx), nat.ptr(dw),
-                                                     0 if dw is None else codes[dw.dtype], nat.ptr(db), 0 if db is None else codes[b_dtype],
-                                                     work.data_ptr(), nat.status_ptr(dev), nat.raw_stream(dev)))
+        if m:
+            columns = need_w or db is not None
+            work = _bytes((_packing_bytes(m, n) if need_x else 0) + (_packing_bytes(n, m) + 4 * n * _ceil128(m) if columns else 0), grad)
+            g = rows_of(grad, n)
+            codes = nat._CODES
+            with nat.on(dev):
+                nat.check(nat.lib().nvfp4_fp8_linear_bwd(g.data_ptr(), codes[g.dtype], m, n, k, pitch_of(g), nat.ptr(x_t), nat.ptr(w_t), nat.ptr(dx),
+                                                         nat.ptr(dw), 0 if dw is None else codes[dw.dtype], nat.ptr(db), 0 if db is None else codes[b_dtype],
+                                                         work.data_ptr(), nat.status_ptr(dev), nat.raw_stream(dev)))
+        else:                # no rows: zeros, handed on like any other gradient (the other ranks' collectives count on it)
+            for t in (dw, db):
+                if t is not None:
+                    t.zero_()
         if taken is not None:
             taken(dw)
             dw = None
