@@ -84,6 +84,11 @@ class AdamW(torch.optim.Optimizer):
     def _grad_mul(self):
         return 1.0 if self.reducer is None else self.reducer.grad_scale
 
+    @staticmethod
+    def _beside(p, pack):
+        """The gradient that autograd left beside a collected one, as the kernels read it: FP32 (autograd holds it in p's dtype)."""
+        return None if pack is None or p.grad is None else p.grad.float()
+
     # ---- updates overlapped with the rest of backward (captured steps) ------------------------------------
     #: Under capture, parameter updates are recorded on a second stream that forks after the parameter's gradient is
     #: complete and joins at the end of backward.  The AdamW kernel is bound by integer / FP32 instruction issue and
@@ -156,7 +161,7 @@ class AdamW(torch.optim.Optimizer):
                 nat.adamw_step(p, 32, grad, s['m'], s['v'], s['ms'], s['vs'], vbits=16, mbits=8, nonlinear_m=False, state_block=BLOCK,
                                hyper=self._hyper(g, t), step=t, key=0, grad_kind=2 if scaled else None,
                                grad_cols=p.shape[-1] if scaled else 1, grad_stride=grad.shape[-1] if scaled else 1, sa=sa, sb=sb,
-                               extra=p.grad if (pack is not None and p.grad is not None) else None, grad_mul=self._grad_mul(),
+                               extra=self._beside(p, pack), grad_mul=self._grad_mul(),
                                ctrl=ctrl, scale_out=scale)
                 torch.autograd.graph.increment_version(p)
                 if cache:
@@ -361,7 +366,7 @@ class AdamW6(AdamW):
                                    nonlinear_m=nonlinear, state_block=g['state_block'], hyper=self._hyper(g, t), step=t,
                                    key=self.keys[p], grad_kind=2 if scaled else None, grad_cols=p.shape[-1] if scaled else 1,
                                    grad_stride=grad.shape[-1] if scaled else 1, sa=sa, sb=sb,
-                                   extra=p.grad if (pack is not None and p.grad is not None) else None, grad_mul=self._grad_mul(),
+                                   extra=self._beside(p, pack), grad_mul=self._grad_mul(),
                                    tail=s.get('tail'), ctrl=ctrl, scale_out=scale)
             torch.autograd.graph.increment_version(p)
             emit['version'] = p._version
@@ -373,7 +378,7 @@ class AdamW6(AdamW):
                        nonlinear_m=g['format'].endswith('_sqrt'), state_block=g['state_block'], hyper=self._hyper(g, t), step=t,
                        key=self.keys[p], grad_kind=2 if scaled else None, grad_cols=p.shape[-1] if scaled else 1,
                        grad_stride=grad.shape[-1] if scaled else 1, sa=sa, sb=sb,
-                       extra=p.grad if (pack is not None and p.grad is not None) else None, grad_mul=self._grad_mul(),
+                       extra=self._beside(p, pack), grad_mul=self._grad_mul(),
                        tail=s.get('tail'), unit=getattr(p, '_v6_unit', None), ctrl=ctrl, scale_out=scale)
         torch.autograd.graph.increment_version(p)
         s['step'] = t
