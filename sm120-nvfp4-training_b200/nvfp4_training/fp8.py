@@ -146,8 +146,8 @@ def _weight_gradient_into(weight):
         return new(weight.dtype), None
     reducer = getattr(weight, "_dp_reducer", None)
     if reducer is not None:
-        if weight in sink:
-            raise RuntimeError("An 8-bit layer may be applied only once per step under data parallel")
+        if weight in sink:             # applied again: the slot is on its way to the other ranks, and this part goes to autograd
+            return new(weight.dtype), None
         slot = reducer.slot(weight)
 
         def reduce(_):

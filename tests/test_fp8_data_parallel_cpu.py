@@ -75,3 +75,35 @@ def _two_ranks(worker):
 
 def test_rank_without_rows_takes_part_in_the_collectives():
     _two_ranks(_no_rows_worker)
+
+
+def _twice_worker(rank, world, port, results):
+    try:
+        fp8, GradientReducer = _begin(rank, world, port)
+        weight = torch.nn.Parameter(torch.zeros(64, 80, dtype=torch.bfloat16))
+        weight._v6_defer_dense = True
+        reducer = GradientReducer([weight])
+        pending = _collecting([weight], reducer)
+        parts = []
+        for value in (1.0, 10.0, 100.0):                    # three applications of the layer in one step
+            into, taken = fp8._weight_gradient_into(weight)
+            into.fill_(value * (rank + 1))
+            if taken is None:
+                assert into.dtype == weight.dtype and into.shape == weight.shape
+                parts.append(into)                          # autograd adds up what it is given
+            else:
+                taken(into)
+        assert len(parts) == 2 and pending[weight][0] is reducer.slot(weight)
+        weight.grad = sum(parts)
+        reducer.finish([weight])
+        assert bool((reducer.slot(weight) == 3).all()) and bool((weight.grad == 330).all())
+        results[rank] = "ok"
+    except Exception as e:  # pragma: no cover - reported to the parent
+        results[rank] = repr(e)
+    finally:
+        dist.destroy_process_group()
+
+
+def test_layer_applied_more_than_once():
+    """The slot takes the first gradient, autograd the others, as for the NVFP4 layers; the optimizer adds the two."""
+    _two_ranks(_twice_worker)
