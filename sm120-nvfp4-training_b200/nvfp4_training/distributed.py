@@ -1,8 +1,8 @@
 """Data-parallel training: replicas that all-reduce weight gradients over NCCL (NVLink / NVSwitch).
 
 The reference is single-GPU; this module is new.  Design:
-  * every converted layer owns a persistent flat BF16 gradient slot; the wgrad GEMM's epilogue writes the scaled
-    gradient straight into it (no pack / copy kernel between GEMM and collective);
+  * every converted layer owns a persistent flat BF16 gradient slot (FP32 for an 8-bit layer with an FP32 master); the wgrad
+    GEMM's epilogue writes the scaled gradient straight into it (no pack / copy kernel between GEMM and collective);
   * a slot is all-reduced asynchronously as soon as its layer's backward has produced it, in backward order, so the
     transfer overlaps the remaining backward compute (NCCL runs on its own stream; only the consumer waits);
   * the fused AdamW kernel reads the reduced slot in place and folds the 1/world_size into its gradient decode;
@@ -43,7 +43,9 @@ class GradientReducer:
         owners = [p for p in params if (owner_filter(p) if owner_filter else getattr(p, "_v4_request_scale", False) or
                                         (getattr(p, "_v6_defer_dense", False) and p.numel() >= 4096))]
         for p in owners:
-            self._slots[p] = torch.zeros(p.numel(), dtype=slot_dtype, device=p.device)
+            # an 8-bit layer with an FP32 master has an FP32 gradient without data parallel, and keeps it here
+            wide = p.dtype == torch.float32 and not getattr(p, "_v4_request_scale", False) and getattr(p, "_v6_defer_dense", False)
+            self._slots[p] = torch.zeros(p.numel(), dtype=torch.float32 if wide else slot_dtype, device=p.device)
         self._works = []          # eager mode: outstanding collectives
         self._queue = deque()     # capture / streaming mode: (param, group, pack, work) waiting for their collective
         self.launched = []        # order in which slots were reduced (introspection / tests)
@@ -160,8 +162,8 @@ class GradientReducer:
 
 
     def layout(self):
-        """What has to agree across ranks for the collectives to pair up: slot sizes in order, bucket size, depth."""
-        return (tuple(t.numel() for t in self._slots.values()), str(self.slot_dtype), self.bucket_bytes, self.depth)
+        """What has to agree across ranks for the collectives to pair up: slot sizes and types in order, bucket size, depth."""
+        return (tuple(t.numel() for t in self._slots.values()), tuple(str(t.dtype) for t in self._slots.values()), self.bucket_bytes, self.depth)
 
 
 def _gather(value, group):

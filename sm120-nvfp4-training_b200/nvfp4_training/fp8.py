@@ -155,6 +155,8 @@ def _weight_gradient_into(weight):
             reducer.ready(weight)
         return slot.view(weight.shape), reduce
 
+    # FP32 for FP32 masters.  For 16-bit ones BF16, FP16 masters included: the update reads either, 2^-9 of a gradient is far below
+    # the noise of its e4m3 operands, and FP16 would lose what is smaller than 6e-8.
     def keep(dw):                                       # a layer applied twice: the sum stays in FP32
         sink[weight] = (dw.add_(sink[weight][0]) if weight in sink else dw, None, None)
     return new(torch.float32 if weight in sink or weight.dtype == torch.float32 else torch.bfloat16), keep

@@ -107,3 +107,20 @@ def _twice_worker(rank, world, port, results):
 def test_layer_applied_more_than_once():
     """The slot takes the first gradient, autograd the others, as for the NVFP4 layers; the optimizer adds the two."""
     _two_ranks(_twice_worker)
+
+
+def test_slots_have_the_gradients_types(tmp_path):
+    from nvfp4_training.distributed import GradientReducer
+    dist.init_process_group("gloo", init_method=f"file://{tmp_path}/store", rank=0, world_size=1)
+    try:
+        nvfp4, *fp8 = (torch.nn.Parameter(torch.zeros(5000, dtype=t)) for t in (torch.float32, torch.float32, torch.float16, torch.bfloat16))
+        nvfp4._v4_request_scale = True
+        for p in fp8:
+            p._v6_defer_dense = True
+        reducer = GradientReducer([nvfp4, *fp8])
+        assert [reducer.slot(p).dtype for p in (nvfp4, *fp8)] == [torch.bfloat16, torch.float32, torch.bfloat16, torch.bfloat16]
+        # ranks whose slots have one size but two types would pair wrong buffers
+        wide, narrow = GradientReducer(fp8[:1]).layout(), GradientReducer(fp8[1:2]).layout()
+        assert wide[0] == narrow[0] and wide != narrow
+    finally:
+        dist.destroy_process_group()
