@@ -234,8 +234,6 @@ _STRIDES = struct.Struct("=qqq")
 @lru_cache(maxsize=256)
 def _plan(sections, dim, theta, layout, frequencies):
     """Checked once per set of arguments: (host arrays of frequency / (2 pi) and axis of every pair, pairs), axes, interleaved."""
-    if not sections or any(type(n) is not int or n < 1 for n in sections):
-        raise ValueError("sections must be positive integers: the pairs of a head that each position axis turns")
     pairs = sum(sections)
     if 2 * pairs > dim or pairs > MAX_PAIRS:
         raise ValueError(f"sections hold {pairs} pairs; a head of {dim} features has room for {min(dim // 2, MAX_PAIRS)}")
@@ -334,7 +332,10 @@ class _RotaryFused(torch.autograd.Function):
 
 
 def _check_rotary(x, batch, seq, dim, positions, sections, theta, layout, frequencies):
-    how = _plan(tuple(sections), dim, float(theta), layout, frequencies)
+    sections = tuple(sections)
+    if not sections or any(type(n) is not int or n < 1 for n in sections):         # not in _plan: 8.0 and True find the entries of 8 and 1
+        raise ValueError("sections must be positive integers: the pairs of a head that each position axis turns")
+    how = _plan(sections, dim, float(theta), layout, frequencies)
     _check_tensor("positions", positions, _POSITION_KINDS)
     shape = positions.shape
     if positions.requires_grad:

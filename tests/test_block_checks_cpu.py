@@ -70,3 +70,12 @@ def test_layer_norm_module_holds_its_shape(without_kernels, affine):
     swapped.__class__ = nv.LayerNorm
     with pytest.raises(ValueError):
         swapped(torch.ones(3, 16))
+
+
+def test_sections_are_integers_also_after_a_call_that_they_equal(without_kernels):
+    q, pos = torch.ones(1, 3, 2, 16), torch.zeros(3, 1)
+    nv.rotary_axes(q, None, pos, (8,))
+    nv.rotary_axes(q, None, pos, (1,))
+    for sections in ((8.0,), (True,), (torch.tensor(8),)):
+        with pytest.raises(ValueError):
+            nv.rotary_axes(q, None, pos, sections)
