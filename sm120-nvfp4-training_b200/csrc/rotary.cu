@@ -195,6 +195,7 @@ extern "C" int nvfp4_rotary_axes(const nvfp4_rotary_tensor* tensors, int count, 
         }
     }
     a.first[3] = heads;
+    NVFP4_REQUIRE(static_cast<int64_t>(heads) * dim < (1LL << 30), NVFP4_ERR_ARG, "nvfp4_rotary_axes: the heads of a token must have fewer than 2^30 features in all");
     for (int j = 0; j < pairs; ++j) {
         NVFP4_REQUIRE(axis[j] < axes, NVFP4_ERR_ARG, "nvfp4_rotary_axes: a pair names an axis that the positions do not have");
         a.turns[j] = turns[j];

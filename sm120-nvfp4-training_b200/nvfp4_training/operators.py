@@ -225,6 +225,7 @@ class LayerNorm(nn.LayerNorm):
 # ---- rotary positions over several axes -----------------------------------------------------------------------------------
 _POSITION_KINDS = {torch.int64: 0, torch.int32: 1, torch.float32: 2, torch.float64: 3}
 MAX_PAIRS = 256
+MAX_TOKEN = 1 << 30        # features of a token's heads, which the kernel counts in 32 bits
 
 
 _JOB = struct.Struct("=QQqqqqqqii")       # nvfp4_rotary_tensor
@@ -331,7 +332,9 @@ class _RotaryFused(torch.autograd.Function):
         return (dqkv if amax is None else attach_amax(dqkv, amax)), None, None, None, None
 
 
-def _check_rotary(x, batch, seq, dim, positions, sections, theta, layout, frequencies):
+def _check_rotary(x, batch, seq, heads, dim, positions, sections, theta, layout, frequencies):
+    if heads * dim >= MAX_TOKEN:
+        raise ValueError(f"the heads of a token must have fewer than {MAX_TOKEN} features in all")
     sections = tuple(sections)
     if not sections or any(type(n) is not int or n < 1 for n in sections):         # not in _plan: 8.0 and True find the entries of 8 and 1
         raise ValueError("sections must be positive integers: the pairs of a head that each position axis turns")
@@ -366,7 +369,7 @@ def rotary_axes(q, k, positions, sections, *, theta=10000.0, layout="half", freq
             raise ValueError("k needs at least one head")
     if q.shape[2] == 0:
         raise ValueError("q needs at least one head")
-    how = _check_rotary(q, q.shape[0], q.shape[1], q.shape[3], positions, sections, theta, layout, frequencies)
+    how = _check_rotary(q, q.shape[0], q.shape[1], q.shape[2] + (0 if k is None else k.shape[2]), q.shape[3], positions, sections, theta, layout, frequencies)
     if not _autograd_sees(q, k):
         return tuple(_turn((q, k), positions, how, False))
     return _RotaryAxes.apply(q, k, positions, how)
@@ -382,7 +385,7 @@ def rotary_axes_qkv(qkv, positions, sections, heads, kv_heads=None, *, theta=100
     if qkv.ndim != 3 or qkv.shape[2] == 0 or qkv.shape[2] % (heads + 2 * kv_heads):
         raise ValueError("qkv must be [batch, seq, (heads + 2 * kv_heads) * dim]")
     dim = qkv.shape[2] // (heads + 2 * kv_heads)
-    how = _check_rotary(qkv, qkv.shape[0], qkv.shape[1], dim, positions, sections, theta, layout, frequencies)
+    how = _check_rotary(qkv, qkv.shape[0], qkv.shape[1], heads + 2 * kv_heads, dim, positions, sections, theta, layout, frequencies)
     qkv = _features_contiguous(qkv)
     if not _autograd_sees(qkv):
         q, k, v = _split_heads(qkv, heads, kv_heads)

@@ -79,3 +79,27 @@ def test_sections_are_integers_also_after_a_call_that_they_equal(without_kernels
     for sections in ((8.0,), (True,), (torch.tensor(8),)):
         with pytest.raises(ValueError):
             nv.rotary_axes(q, None, pos, sections)
+
+
+def test_rotary_refuses_tokens_beyond_its_counters(without_kernels):
+    """The kernel counts the features of a token's heads in 32 bits."""
+    one, pos = torch.ones(1), torch.zeros(1, 1)
+    heads = lambda h, d: one.expand(1, 1, h, d)
+    for q, k in ((heads(1 << 20, 1 << 10), None), (heads(1 << 19, 1 << 10), heads(1 << 19, 1 << 10)), (heads(1, 1 << 30), None), (heads(1 << 31, 2), None)):
+        with pytest.raises(ValueError, match="features"):
+            nv.rotary_axes(q, k, pos, (1,))
+    with pytest.raises(ValueError, match="features"):
+        nv.rotary_axes_qkv(one.expand(1, 1, 3 << 29), pos, (1,), 1)
+
+
+def test_rotary_entry_point_refuses_tokens_beyond_its_counters():
+    import ctypes as C
+    from nvfp4_training import _native
+    lib = _native.lib()
+    buf = C.create_string_buffer(64)
+    at = (C.addressof(buf) + 15) // 16 * 16
+    turns, axis, strides = (C.c_double * 1)(), (C.c_uint8 * 1)(), (C.c_int64 * 3)()
+    for count, heads, dim in ((1, 1 << 19, 1 << 11), (3, 1 << 19, 1 << 10), (3, (1 << 20) - 1, (1 << 31) - 2)):
+        tensors = operators._JOB.pack(at, at, 0, 0, 0, 0, 0, 0, heads, 1) * count
+        assert lib.nvfp4_rotary_axes(tensors, count, 1, 1, 1, dim, buf, 0, strides, 1, turns, axis, 1, 0, 0, None, None) == 1
+        assert b"features" in lib.nvfp4_last_error()
