@@ -269,7 +269,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             const uint32_t lane_at = tmem_base + (static_cast<uint32_t>(sub * 32) << 16);
             if constexpr (!CHUNKS) {       // drain to packed registers, then store
                 const int acc = local & 1;
-                if (!mbar_wait(&acc_full[acc], (local >> 1) & 1, abort_flag)) { ok = false; break; }
+                if (!mbar_wait_warp(&acc_full[acc], (local >> 1) & 1, abort_flag)) { ok = false; break; }
                 tc_fence_after();
                 // unit i of this warp: the shared one first (the last two of stage 0, the first two of stage 1), then seven of its own
                 auto unit_of = [&](int i) { return i == 0 ? (acc == 0 ? 14 + half : half) : (acc == 0 ? 0 : 2) + half * 7 + (i - 1); };
@@ -299,7 +299,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 float sum[8][16];
                 for (int k0 = 0; k0 < g.k_tiles; k0 += CHUNK<TO>, ++local) {
                     const int acc = local & 1;
-                    if (!mbar_wait(&acc_full[acc], (local >> 1) & 1, abort_flag)) { ok = false; break; }
+                    if (!mbar_wait_warp(&acc_full[acc], (local >> 1) & 1, abort_flag)) { ok = false; break; }
                     tc_fence_after();
                     // the shared columns are the last two units of stage 0 (the upper half's) and the first two of stage 1 (the lower's)
                     const bool holds_shared = half != acc;

@@ -328,7 +328,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             const int tm = (t % g.tiles_m) * Cfg::CTAS + rank, tn = t / g.tiles_m;
             const int acc = local & 1;
             const uint32_t acc_phase = (local >> 1) & 1;
-            if (!mbar_wait(&acc_full[acc], acc_phase, abort_flag)) { ok = false; break; }
+            if (!mbar_wait_warp(&acc_full[acc], acc_phase, abort_flag)) { ok = false; break; }
             tc_fence_after();
             const int64_t row = static_cast<int64_t>(tm) * BM + row_in_tile;
             const int tile_row0 = tm * BM + sub * 32;
