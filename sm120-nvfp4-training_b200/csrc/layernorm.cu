@@ -776,7 +776,7 @@ __global__ void __launch_bounds__(MAXT, CTAS) norm_bwd_ring_kernel(const NormBwd
     }
 }
 
-constexpr int64_t NORM_MAX_PARTS = 148 * 6;
+constexpr int64_t SMS = 148;
 constexpr int64_t MAX_GRID = 1 << 30;
 
 static int round32(int n) { return (n + 31) / 32 * 32; }
@@ -786,10 +786,25 @@ static int round32(int n) { return (n + 31) / 32 * 32; }
 // backward); below, the rows would not fill a warp.  Narrow rows stand in groups that make 256 threads.  As many CTAs per SM
 // as the registers allow and as leave each of them three stages.
 static int columns_per_thread(int64_t cols) { return cols >= 2048 ? 16 : 8; }
+static int round_threads(int64_t cols) { return round32(static_cast<int>((cols + columns_per_thread(cols) - 1) / columns_per_thread(cols))); }
+static int bwd_threads_per_sm(int64_t cols) { return columns_per_thread(cols) == 8 ? 512 : 640; }
+
+// Partial rows of dw and db at most, which is what the caller's scratch holds: every way the backward pass may go at this width
+// keeps to it.  Wide rows are summed by a pass of their own, in about 16 CTAs per SM of 32 columns each.
+static int64_t column_pass_parts(int64_t rows, int64_t cols) {
+    return std::min<int64_t>({(rows + 31) / 32, SMS * 4, std::max<int64_t>(1, SMS * 16 / ((cols + 31) / 32))});
+}
+static int64_t bwd_parts_limit(int64_t rows, int64_t cols) {
+    if (cols > 8192) return column_pass_parts(rows, cols);
+    const int row_threads = round_threads(cols), threads = row_threads * std::max(1, 256 / row_threads);
+    const int64_t ring = SMS * std::max(1, bwd_threads_per_sm(cols) / threads);
+    const int64_t other = cols <= 768 ? SMS * 2 : cols <= 4096 ? SMS * 3 : column_pass_parts(rows, cols);
+    return std::min(rows, std::max(ring, other));
+}
 static ring::Plan ring_plan(int64_t rows, int64_t cols, int rows_per_group, int row_bytes, int sms, int threads_per_sm, bool backward) {
     ring::Plan p;
     const int per_thread = columns_per_thread(cols);
-    p.row_threads = round32(static_cast<int>((cols + per_thread - 1) / per_thread));
+    p.row_threads = round_threads(cols);
     // few rows: no group without one
     const int64_t want = std::max<int64_t>(1, (rows + static_cast<int64_t>(rows_per_group) * sms - 1) / (static_cast<int64_t>(rows_per_group) * sms));
     const int groups = static_cast<int>(std::min<int64_t>(std::max(1, 256 / p.row_threads), want));
@@ -802,7 +817,7 @@ static ring::Plan ring_plan(int64_t rows, int64_t cols, int rows_per_group, int 
     // the groups' column sums of the backward pass (8 bytes a column) meet in the stages
     if (backward) while (p.stages * p.stage_bytes < groups * 8 * cols) ++p.stages;
     const int64_t all = (rows + static_cast<int64_t>(groups) * rows_per_group - 1) / (static_cast<int64_t>(groups) * rows_per_group);
-    p.ctas = static_cast<int>(std::min<int64_t>({all, static_cast<int64_t>(p.ctas) * sms, NORM_MAX_PARTS}));
+    p.ctas = static_cast<int>(std::min<int64_t>({all, static_cast<int64_t>(p.ctas) * sms, backward ? bwd_parts_limit(rows, cols) : all}));
     return p;
 }
 static bool ring_operand(const void* p, int dtype, int64_t pitch, int64_t cols) {       // rows that bulk copies can fetch
@@ -852,8 +867,8 @@ template <typename TX, typename TH>
 static int64_t bwd_ring_sized(const NormBwdArgs& a, cudaStream_t st) {
     const int row_bytes = a.cols * static_cast<int>(sizeof(TH) + sizeof(TX) * (a.dsum ? 2 : 1));
     if (columns_per_thread(a.cols) == 8)
-        return bwd_ring<TX, TH, 8, 2, 256, 2>(a, ring_plan(a.rows, a.cols, 2, row_bytes, sm_count(), 512, true), st);
-    const ring::Plan p = ring_plan(a.rows, a.cols, 1, row_bytes, sm_count(), 640, true);
+        return bwd_ring<TX, TH, 8, 2, 256, 2>(a, ring_plan(a.rows, a.cols, 2, row_bytes, sm_count(), bwd_threads_per_sm(a.cols), true), st);
+    const ring::Plan p = ring_plan(a.rows, a.cols, 1, row_bytes, sm_count(), bwd_threads_per_sm(a.cols), true);
     if (p.threads <= 256) return bwd_ring<TX, TH, 16, 1, 256, 2>(a, p, st);
     return p.threads <= 320 ? bwd_ring<TX, TH, 16, 1, 320, 2>(a, p, st) : bwd_ring<TX, TH, 16, 1, 512, 1>(a, p, st);
 }
@@ -885,7 +900,7 @@ static int64_t backward(const NormBwdArgs& a, bool ring, cudaStream_t st) {
     if (ring)
         if (const int64_t parts = bwd_ring_sized<TX, TH>(a, st)) return parts;
     auto by_warp = [&](auto kernel) {
-        const int64_t parts = std::min<int64_t>((a.rows + 7) / 8, 148 * 2);
+        const int64_t parts = std::min<int64_t>((a.rows + 7) / 8, SMS * 2);
         kernel<<<static_cast<unsigned>(parts), 256, 0, st>>>(a);
         return parts;
     };
@@ -893,15 +908,14 @@ static int64_t backward(const NormBwdArgs& a, bool ring, cudaStream_t st) {
     if (a.cols <= 768) return by_warp(norm_bwd_kernel<TX, TH, 24, false>);
     if (a.cols <= 4096) {
         const int threads = round32((a.cols + 7) / 8);
-        const int64_t parts = std::min<int64_t>(a.rows, 148 * (threads <= 256 ? 3 : threads <= 384 ? 2 : 1));
+        const int64_t parts = std::min<int64_t>(a.rows, SMS * (threads <= 256 ? 3 : threads <= 384 ? 2 : 1));
         norm_bwd_kernel<TX, TH, 8, true><<<static_cast<unsigned>(parts), threads, 0, st>>>(a);
         return parts;
     }
     norm_bwd_any_kernel<TX, TH><<<static_cast<unsigned>(std::min(a.rows, MAX_GRID)), 256, 0, st>>>(a);
     if (!a.partial) return 1;
-    const int64_t blocks = (a.cols + 31) / 32;
-    const int64_t parts = std::min<int64_t>({(a.rows + 31) / 32, static_cast<int64_t>(592), std::max<int64_t>(1, 148 * 16 / blocks)});
-    norm_bwd_columns_kernel<TX, TH><<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(parts)), 256, 0, st>>>(a);
+    const int64_t parts = column_pass_parts(a.rows, a.cols);
+    norm_bwd_columns_kernel<TX, TH><<<dim3(static_cast<unsigned>((a.cols + 31) / 32), static_cast<unsigned>(parts)), 256, 0, st>>>(a);
     return parts;
 }
 
@@ -938,7 +952,9 @@ extern "C" int nvfp4_layer_norm(const void* x, int x_dtype, int64_t x_pitch, con
     return launch_status("nvfp4_layer_norm");
 }
 
-extern "C" int64_t nvfp4_layer_norm_bwd_partials(int64_t rows, int64_t) { return std::max<int64_t>(1, std::min(rows, NORM_MAX_PARTS)); }
+extern "C" int64_t nvfp4_layer_norm_bwd_partials(int64_t rows, int64_t cols) {
+    return rows > 0 && cols > 0 ? std::max<int64_t>(1, bwd_parts_limit(rows, std::min<int64_t>(cols, 1 << 30))) : 1;
+}
 
 extern "C" int nvfp4_layer_norm_bwd(const void* dh, int h_dtype, int64_t dh_pitch, const void* total, int x_dtype, int64_t total_pitch,
                                     const float* mean, const float* rstd, const void* weight, int weight_dtype, const void* dsum,

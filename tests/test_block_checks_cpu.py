@@ -103,3 +103,12 @@ def test_rotary_entry_point_refuses_tokens_beyond_its_counters():
         tensors = operators._JOB.pack(at, at, 0, 0, 0, 0, 0, 0, heads, 1) * count
         assert lib.nvfp4_rotary_axes(tensors, count, 1, 1, 1, dim, buf, 0, strides, 1, turns, axis, 1, 0, 0, None, None) == 1
         assert b"features" in lib.nvfp4_last_error()
+
+
+@pytest.mark.parametrize("cols", [1, 64, 768, 1027, 2048, 4096, 5120, 8192, 8200, 16400, 131072, 1 << 20, (1 << 30) - 1])
+@pytest.mark.parametrize("rows", [1, 40, 1024, 16384, 10 ** 7])
+def test_layer_norm_scratch_is_what_the_width_uses(cols, rows):
+    """Partial sums of the parameters' gradients: one row at least, never more than the rows there are, and 16 MB or one row of them."""
+    from nvfp4_training import _native
+    parts = _native.lib().nvfp4_layer_norm_bwd_partials(rows, cols)
+    assert 1 <= parts <= rows and parts * 2 * cols * 4 <= max(16 << 20, 8 * cols)
