@@ -783,8 +783,11 @@ static int round32(int n) { return (n + 31) / 32 * 32; }
 
 // Sixteen columns a thread from 2048 columns on, eight below: a round costs a thread about 150 instructions whatever it holds
 // (waiting, two reductions, addresses), which sixteen columns halve (16384 x 5120 BF16: 179 -> 109 us forward, 165 -> 137
-// backward); below, the rows would not fill a warp.  Narrow rows stand in groups that make 256 threads.  As many CTAs per SM
-// as the registers allow and as leave each of them three stages.
+// backward when it was made); below, the rows would not fill a warp.  Narrow rows stand in groups that make 256 threads.  As many
+// CTAs per SM as the registers allow (threads_that_fit) and as leave each of them three stages, within a budget of threads: 1024
+// forward and 512 backward with eight columns a thread, 640 with sixteen.  A CTA more than fits would run behind the others with
+// its share of the rows, on stages cut to its size: backward, 2304 columns BF16 (160 threads of 128 registers), 159 us with four
+// CTAs planned, 112 with the three that fit.
 static int columns_per_thread(int64_t cols) { return cols >= 2048 ? 16 : 8; }
 static int round_threads(int64_t cols) { return round32(static_cast<int>((cols + columns_per_thread(cols) - 1) / columns_per_thread(cols))); }
 static int bwd_threads_per_sm(int64_t cols) { return columns_per_thread(cols) == 8 ? 512 : 640; }
@@ -831,6 +834,15 @@ static int sm_count() {
     if (!count[dev]) cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev);
     return count[dev];
 }
+// Threads of KERNEL that the registers of an SM hold (allocated by eights a thread), asked once per kernel; 512 at 128 registers.
+template <typename Args>
+static int threads_that_fit(void (*kernel)(Args, int, int), int& known) {
+    if (!known) {
+        cudaFuncAttributes f;
+        known = cudaFuncGetAttributes(&f, kernel) == cudaSuccess && f.numRegs > 0 ? 65536 / ((f.numRegs + 7) / 8 * 8) : 512;
+    }
+    return known;
+}
 // One launch of a ring kernel; KERNEL's shared-memory limit is raised once per device.
 template <typename Args>
 static bool launch_ring(void (*kernel)(Args, int, int), bool (&ready)[64], const Args& a, const ring::Plan& p, cudaStream_t st) {
@@ -845,32 +857,37 @@ static bool launch_ring(void (*kernel)(Args, int, int), bool (&ready)[64], const
     return true;
 }
 template <typename TX, typename TD, typename TO, int C, int R, int MAXT, int CTAS>
-static bool fwd_ring(const NormArgs& a, const ring::Plan& p, cudaStream_t st) {
+static bool fwd_ring(const NormArgs& a, int row_bytes, int threads_per_sm, cudaStream_t st) {
     static bool ready[64] = {};
-    return launch_ring<NormArgs>(norm_fwd_ring_kernel<TX, TD, TO, C, R, MAXT, CTAS>, ready, a, p, st);
+    static int fit = 0;
+    const auto kernel = norm_fwd_ring_kernel<TX, TD, TO, C, R, MAXT, CTAS>;
+    const ring::Plan p = ring_plan(a.rows, a.cols, R, row_bytes, sm_count(), std::min(threads_per_sm, threads_that_fit<NormArgs>(kernel, fit)), false);
+    return launch_ring<NormArgs>(kernel, ready, a, p, st);
 }
 template <typename TX, typename TD, typename TO>
 static bool fwd_ring_sized(const NormArgs& a, cudaStream_t st) {
     const int row_bytes = a.cols * static_cast<int>(sizeof(TX) + (a.delta ? sizeof(TD) : 0));
-    if (columns_per_thread(a.cols) == 8)
-        return fwd_ring<TX, TD, TO, 8, 2, 256, 4>(a, ring_plan(a.rows, a.cols, 2, row_bytes, sm_count(), 1024, false), st);
-    const ring::Plan p = ring_plan(a.rows, a.cols, 1, row_bytes, sm_count(), 640, false);
-    if (p.threads <= 256) return fwd_ring<TX, TD, TO, 16, 1, 256, 2>(a, p, st);
-    return p.threads <= 320 ? fwd_ring<TX, TD, TO, 16, 1, 320, 2>(a, p, st) : fwd_ring<TX, TD, TO, 16, 1, 512, 1>(a, p, st);
+    const int row_threads = round_threads(a.cols);
+    if (columns_per_thread(a.cols) == 8) return fwd_ring<TX, TD, TO, 8, 2, 256, 4>(a, row_bytes, 1024, st);
+    if (row_threads <= 256) return fwd_ring<TX, TD, TO, 16, 1, 256, 2>(a, row_bytes, 640, st);
+    return row_threads <= 320 ? fwd_ring<TX, TD, TO, 16, 1, 320, 2>(a, row_bytes, 640, st) : fwd_ring<TX, TD, TO, 16, 1, 512, 1>(a, row_bytes, 640, st);
 }
 template <typename TX, typename TH, int C, int R, int MAXT, int CTAS>
-static int64_t bwd_ring(const NormBwdArgs& a, const ring::Plan& p, cudaStream_t st) {
+static int64_t bwd_ring(const NormBwdArgs& a, int row_bytes, cudaStream_t st) {
     static bool ready[64] = {};
-    return launch_ring<NormBwdArgs>(norm_bwd_ring_kernel<TX, TH, C, R, MAXT, CTAS>, ready, a, p, st) ? p.ctas : 0;
+    static int fit = 0;
+    const auto kernel = norm_bwd_ring_kernel<TX, TH, C, R, MAXT, CTAS>;
+    const int threads = std::min(bwd_threads_per_sm(a.cols), threads_that_fit<NormBwdArgs>(kernel, fit));
+    const ring::Plan p = ring_plan(a.rows, a.cols, R, row_bytes, sm_count(), threads, true);
+    return launch_ring<NormBwdArgs>(kernel, ready, a, p, st) ? p.ctas : 0;
 }
 template <typename TX, typename TH>
 static int64_t bwd_ring_sized(const NormBwdArgs& a, cudaStream_t st) {
     const int row_bytes = a.cols * static_cast<int>(sizeof(TH) + sizeof(TX) * (a.dsum ? 2 : 1));
-    if (columns_per_thread(a.cols) == 8)
-        return bwd_ring<TX, TH, 8, 2, 256, 2>(a, ring_plan(a.rows, a.cols, 2, row_bytes, sm_count(), bwd_threads_per_sm(a.cols), true), st);
-    const ring::Plan p = ring_plan(a.rows, a.cols, 1, row_bytes, sm_count(), bwd_threads_per_sm(a.cols), true);
-    if (p.threads <= 256) return bwd_ring<TX, TH, 16, 1, 256, 2>(a, p, st);
-    return p.threads <= 320 ? bwd_ring<TX, TH, 16, 1, 320, 2>(a, p, st) : bwd_ring<TX, TH, 16, 1, 512, 1>(a, p, st);
+    const int row_threads = round_threads(a.cols);
+    if (columns_per_thread(a.cols) == 8) return bwd_ring<TX, TH, 8, 2, 256, 2>(a, row_bytes, st);
+    if (row_threads <= 256) return bwd_ring<TX, TH, 16, 1, 256, 2>(a, row_bytes, st);
+    return row_threads <= 320 ? bwd_ring<TX, TH, 16, 1, 320, 2>(a, row_bytes, st) : bwd_ring<TX, TH, 16, 1, 512, 1>(a, row_bytes, st);
 }
 
 // Rows that bulk copies cannot fetch, or wider than the ring's threads hold: odd widths and unaligned rows element by element in
