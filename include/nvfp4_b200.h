@@ -357,7 +357,8 @@ int nvfp4_layer_norm_bwd(const void* dh, int h_dtype, int64_t dh_pitch, const vo
  * nvfp4_rotary_axes: up to three tensors [batch][seq][heads][dim] (strides of batch, seq and head in elements, features
  *   contiguous) in one launch.  Pair j < pairs of a head turns by position[token][axis[j]] * turns[j] full turns, formed and
  *   reduced in FP64; features from 2 * pairs on, and tensors with turn == 0, are copied.  interleaved: pair j is (2j, 2j + 1),
- *   else (j, j + pairs).  inverse turns the other way (the backward pass).  positions: int64 (position_kind 0), int32 (1),
+ *   else (j, j + pairs).  The angle is off by about |position * frequency| * 2^-52 radians, and by FP32's rounding of its
+ *   remainder.  inverse turns the other way (the backward pass).  positions: int64 (position_kind 0), int32 (1),
  *   FP32 (2) or FP64 (3) with strides of batch, seq and axis in elements.  turns (FP64, frequency / 2 pi) and axis (uint8):
  *   host arrays of `pairs` entries, at most NVFP4_ROTARY_MAX_PAIRS.  The heads of a token have fewer than 2^30 features in all.
  */

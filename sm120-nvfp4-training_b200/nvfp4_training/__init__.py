@@ -64,7 +64,8 @@ def prepare_training(model, *, profile="balanced", precision="fp4", remat=False,
 
     fp8_layers: patterns of Linear layers (their path or an ancestor's, shell style) whose products run in 8 bits instead of
     NVFP4, for layers that do not bear 4; masters and optimizer state keep the profile's format (not with the FP8-master
-    profile).  fused_norms: nn.LayerNorm modules over one dimension run on nvfp4_training.LayerNorm."""
+    profile).  fused_norms: nn.LayerNorm modules over one dimension run on nvfp4_training.LayerNorm, which under BF16
+    autocast turns an FP32 input into a BF16 result (nn.LayerNorm: FP32)."""
     from ._convert import prepare
     return prepare(model, profile=profile, precision=precision, remat=remat, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
                    fp8_layers=fp8_layers, fused_norms=fused_norms)

@@ -355,7 +355,7 @@ def rotary_axes(q, k, positions, sections, *, theta=10000.0, layout="half", freq
     int64, FP32 or FP64; sections: pairs turned by each axis, in order, at most dim / 2 in all (features behind the turned
     ones pass unchanged).  frequencies 'shared': pair j of all P turns by theta^(-j / P), whatever its axis; 'axis': pair i
     of an axis of n pairs by theta^(-i / n).  layout 'half': pair j is features (j, j + P); 'interleaved': (2j, 2j + 1).
-    Angles are FP64."""
+    Angles are FP64: off by about |position * frequency| * 2^-52 radians before sines and cosines are formed in FP32."""
     _check_tensor("q", q)
     if q.ndim != 4:
         raise ValueError("q must be [batch, seq, heads, dim]")
